@@ -224,6 +224,102 @@ FP4X_API int llama_attn_decode_f32q_bf16kv(fp4x_stream_t stream, uint32_t batch,
                                   const uint16_t *kc, const uint16_t *vc, float *out, void *workspace,
                                   size_t workspace_bytes);
 
+/* ------------------------------------------------------------ MX KV cache
+ * No counterpart in the reference (its cache is one f32 array per sequence,
+ * llama_run/src/main.rs:388-389): a paged KV cache held in an OCP MX format, the
+ * attention that reads it, attention over a prefix shared by a batch, and the
+ * verification of drafted tokens that multi-token decode steps end in.
+ *
+ * A cache is described by this struct (plain pointers, owned by the caller).  K and
+ * V have the same layout: codes [n_pages][n_kv][page_size][row bytes] and E8M0
+ * scales [n_pages][n_kv][page_size][head_dim/32], pages page_stride and
+ * scale_page_stride bytes apart (one (page, head) block is contiguous).  A row holds
+ * dimension d = 32 b + 4 g + i (b < head_dim/32, g < 8, i < 4) at code position
+ * (g * head_dim/32 + b) * 4 + i, so that the 16-byte pieces of a row carry the same
+ * four dimensions of every 32-block: the order in which the attention's tensor-core
+ * fragments use them.  MXFP8: one E4M3 byte per code (row bytes = head_dim), scale
+ * 2^(floor(log2 amax) - 8), values beyond 448 saturate, NaN keeps its code 0x7F.
+ * MXFP4: E2M1 nibbles, low nibble first (row bytes = head_dim/2), the scale and
+ * rounding rule of fp4_quantize_mxfp4; a block with a NaN gets scale 255 (NaN).
+ * Infinite values saturate.  A block of zeros has scale 127.
+ * Position t of a sequence is row t % page_size of its page t / page_size; a slot is
+ * page * page_size + row.  k and v 16-byte aligned, page_stride a multiple of 16,
+ * scales 8-byte aligned, scale_page_stride a multiple of 8; head_dim 64 or 128;
+ * page_size 16, 32, 64, 128 or 256; n_pages * page_size < 2^31. */
+typedef enum { FP4X_MXFP8 = 0, FP4X_MXFP4 = 1 } fp4x_mx_format;
+typedef enum { FP4X_F32 = 0, FP4X_BF16 = 1 } fp4x_dtype;
+typedef struct fp4x_mxkv {
+    uint8_t *k, *k_scales, *v, *v_scales;
+    uint64_t page_stride, scale_page_stride; /* bytes */
+    uint32_t n_pages, page_size, n_kv_heads, head_dim, format;
+} fp4x_mxkv;
+
+/* Quantise `n` rows of K and of V ([n][n_kv][head_dim], rows k_stride / v_stride
+ * elements apart, 16-byte aligned) into the slots slots[0..n); a negative slot skips
+ * its row, a slot past the cache skips it and sets the device error word
+ * (fp4x_device_error).  Slots of one call must differ.  Replaces copy_into for this
+ * cache (llama_run/src/main.rs:140-146). */
+FP4X_API int llama_kv_append_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t n, const int32_t *slots,
+                                uint32_t dtype, const void *k, uint64_t k_stride, const void *v, uint64_t v_stride);
+/* Dequantise the rows in slots[0..n) to k_out, v_out [n][n_kv][head_dim] (exact in
+ * both types up to their exponent range); a negative slot gives zeros, as does one
+ * past the cache, which also sets the device error word. */
+FP4X_API int llama_kv_read_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t n, const int32_t *slots,
+                              uint32_t dtype, void *k_out, void *v_out);
+/* Bytes of workspace of the two attention calls below (prefix_len 0 for the first). */
+FP4X_API size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads, uint32_t q_len,
+                                             uint32_t prefix_len, uint32_t max_len);
+/* Decode attention over the paged cache: q [batch][q_len][n_heads][head_dim] (token
+ * rows q_stride elements apart, 16-byte aligned), out the same shape, contiguous and
+ * 16-byte aligned.  Sequence b holds lens[b] positions (device array; clamped to
+ * 0..max_len), the q_len query tokens of this step included as the last ones: query
+ * i attends to positions 0 .. lens[b] - q_len + i.  A query that sees no position
+ * gives zeros.  page_table [batch] rows of table_stride page ids, at least
+ * ceil(max_len / page_size) each; ids outside the cache are not read: their
+ * positions are masked and the device error word is set.  Softmax scale
+ * 1/sqrt(head_dim), statistics and sums in f32; with bf16 q the probabilities enter
+ * the tensor cores as f16, with f32 q both operands as f16 pairs (22 bits).
+ * n_heads a multiple of n_kv_heads. */
+FP4X_API int llama_attn_paged_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
+                                 uint32_t q_len, const int32_t *page_table, uint32_t table_stride,
+                                 const int32_t *lens, uint32_t max_len, uint32_t dtype, const void *q,
+                                 uint64_t q_stride, void *out, void *workspace, size_t workspace_bytes);
+/* The same for a batch whose sequences continue one shared prefix: every query sees
+ * the prefix_len positions behind prefix_pages (device array of
+ * ceil(prefix_len / page_size) ids) first, then its sequence's own positions as
+ * above.  The prefix is read and dequantised once for the rows of all sequences. */
+FP4X_API int llama_attn_shared_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
+                                  uint32_t q_len, const int32_t *prefix_pages, uint32_t prefix_len,
+                                  const int32_t *page_table, uint32_t table_stride, const int32_t *lens,
+                                  uint32_t max_len, uint32_t dtype, const void *q, uint64_t q_stride, void *out,
+                                  void *workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------ speculative decode */
+
+/* Verify up to k drafted tokens per sequence against the target model's logits
+ * [batch][k + 1][vocab] (rows logits_stride elements apart), keeping the target's
+ * distribution exactly (speculative sampling with given random numbers):
+ *   p_i = softmax(logits[b][i] / temperature[b]); draft d_i is accepted while
+ *   uniforms[b][i] * q_i(d_i) < p_i(d_i); at the first rejection the token is
+ *   argmax_v max(p_i(v) - q_i(v), 0) / noise[b][v], after all of them
+ *   argmax_v p_k(v) / noise[b][v] (noise: exponential(1) draws, so this samples).
+ * draft_probs [batch][k][vocab] f32 are the q_i (NULL: the drafts were certain,
+ * q_i = 1 at d_i); draft_lens[b] <= k drafts count (NULL: k); temperature NULL: 1.
+ * A temperature that is not above 1e-30 (0, negative, NaN) decodes greedily: a draft
+ * is accepted if it is the argmax (ties to the lowest index), the last token is the
+ * argmax, uniforms and noise are not used.  NaN logits count as -inf.  A residual or
+ * distribution without any mass falls back to p, then to the argmax.  A draft id
+ * outside the vocabulary is rejected.  Outputs: accepted[b]; tokens [batch][k + 1] =
+ * the accepted drafts, the sampled token, then -1; logprobs (NULL: not wanted) =
+ * log p_i(token_i), at temperature 1 when greedy, 0 past the last token.
+ * Ties of the argmax go to the lowest index. */
+FP4X_API size_t llama_verify_workspace_size(uint32_t batch, uint32_t k, uint32_t vocab);
+FP4X_API int llama_verify_drafts(fp4x_stream_t stream, uint32_t batch, uint32_t k, uint32_t vocab, uint32_t dtype,
+                                 const void *logits, uint64_t logits_stride, const float *draft_probs,
+                                 const int32_t *drafts, const int32_t *draft_lens, const float *uniforms,
+                                 const float *noise, const float *temperature, int32_t *accepted, int32_t *tokens,
+                                 float *logprobs, void *workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------------ decode engine */
 
 /* Model shape + synthetic-init seed.  The reference hard-codes these as consts

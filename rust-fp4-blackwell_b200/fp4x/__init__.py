@@ -77,7 +77,24 @@ SIGNATURES = {
                                                 _vp, _vp, _vp, _vp, _vp, _sz]),
     "llama_attn_decode_bf16_noalloc": (C.c_int, [_vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp]),
     "llama_attn_noalloc_max_bytes": (_sz, []),
+    "llama_kv_append_mx": (C.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u64, _vp, _u64]),
+    "llama_kv_read_mx": (C.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp]),
+    "llama_attn_mx_workspace_size": (_sz, [_vp, _u32, _u32, _u32, _u32, _u32]),
+    "llama_attn_paged_mx": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u64, _vp,
+                                      _vp, _sz]),
+    "llama_attn_shared_mx": (C.c_int, [_vp, _vp, _u32, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _u64,
+                                       _vp, _vp, _sz]),
+    "llama_verify_workspace_size": (_sz, [_u32, _u32, _u32]),
+    "llama_verify_drafts": (C.c_int, [_vp, _u32, _u32, _u32, _u32, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                      _vp, _vp, _sz]),
 }
+
+
+class MxKv(C.Structure):
+    """fp4x_mxkv of the C ABI: pointers and shape of an MX-quantised paged KV cache."""
+    _fields_ = [("k", _vp), ("k_scales", _vp), ("v", _vp), ("v_scales", _vp), ("page_stride", _u64),
+                ("scale_page_stride", _u64), ("n_pages", _u32), ("page_size", _u32), ("n_kv_heads", _u32),
+                ("head_dim", _u32), ("format", _u32)]
 
 
 def lib():

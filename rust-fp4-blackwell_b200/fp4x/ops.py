@@ -3,9 +3,11 @@ tensors and the current torch stream to libfp4x.so.  Tensors must be CUDA and
 contiguous; nothing here computes on the host."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from . import check, lib
+from . import MxKv, check, lib
 
 
 def _stream():
@@ -209,3 +211,179 @@ def attn_decode_bf16(q, kc, vc, seq, split=True):
     check(lib().llama_attn_decode_bf16(_stream(), B, H, n_kv, hd, seq, max_seq, _ptr(q), _ptr(kc), _ptr(vc),
                                        _ptr(out), _ptr(ws) if ws is not None else None, nbytes))
     return out
+
+
+# ------------------------------------------------------------ MX KV cache
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _dtype(t: torch.Tensor) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"fp4x: {t.dtype} is not float32 or bfloat16")
+    return d
+
+
+def _i32(t: torch.Tensor, name: str):
+    if t.dtype != torch.int32:
+        raise ValueError(f"{name} must be int32, not {t.dtype}")
+    return _ptr(t)
+
+
+def _f32(t: torch.Tensor, name: str):
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32, not {t.dtype}")
+    return _ptr(t)
+
+
+def _rows(t: torch.Tensor, n: int, name: str):
+    """Pointer and row stride of [rows][n] data whose leading dimension may be strided."""
+    if not t.is_cuda:
+        raise ValueError("fp4x operators take CUDA tensors (no CPU fallback)")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else n)
+
+
+class MxKvCache:
+    """Paged KV cache in MXFP8 (E4M3) or MXFP4 (E2M1) with one E8M0 scale per 32 values.
+
+    k, v: uint8 [n_pages][n_kv][page_size][head_dim or head_dim/2], k_scales, v_scales: uint8
+    [n_pages][n_kv][page_size][head_dim/32]; the page dimension may be strided (alike for K and V), as in one
+    allocation that holds K and V pages in turn.  Row layout: see fp4x_mxkv in fp4x.h.
+    """
+
+    def __init__(self, k, k_scales, v, v_scales):
+        n_pages, n_kv, page, row = k.shape
+        head_dim = 32 * k_scales.shape[-1]
+        if row not in (head_dim, head_dim // 2):
+            raise ValueError(f"row of {row} bytes does not hold head_dim {head_dim}")
+        if v.shape != k.shape or k_scales.shape != (n_pages, n_kv, page, head_dim // 32) \
+                or v_scales.shape != k_scales.shape:
+            raise ValueError("K, V and their scales disagree in shape")
+        for t in (k, k_scales, v, v_scales):
+            if t.dtype != torch.uint8 or not t.is_cuda or t.device != k.device:
+                raise ValueError("an MX cache is uint8 CUDA tensors of one device")
+            if n_pages and not t[0].is_contiguous():
+                raise ValueError("every page must be contiguous")
+        if n_pages > 1 and (k.stride(0) != v.stride(0) or k_scales.stride(0) != v_scales.stride(0)):
+            raise ValueError("K and V must have the same page stride")
+        self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
+        self.n_pages, self.n_kv, self.page_size, self.head_dim = n_pages, n_kv, page, head_dim
+        self.format = "mxfp8" if row == head_dim else "mxfp4"
+        strides = (k.stride(0), k_scales.stride(0)) if n_pages > 1 else (k[0].numel(), k_scales[0].numel())
+        self._struct = MxKv(k.data_ptr(), k_scales.data_ptr(), v.data_ptr(), v_scales.data_ptr(), *strides, n_pages,
+                            page, n_kv, head_dim, 0 if row == head_dim else 1)
+        self.ptr = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, n_pages, n_kv, head_dim, page_size=64, fmt="mxfp8", device="cuda"):
+        """A cache of `n_pages` pages; nothing is read from a row before it is written."""
+        if fmt not in ("mxfp8", "mxfp4"):
+            raise ValueError(fmt)
+        row = head_dim if fmt == "mxfp8" else head_dim // 2
+        shape = (n_pages, n_kv, page_size)
+        new = [torch.empty(shape + (n,), dtype=torch.uint8, device=device) for n in (row, head_dim // 32) * 2]
+        return cls(*new)
+
+
+def kv_append_mx(cache: MxKvCache, slots, k, v):
+    """Quantise rows k, v [n][n_kv][head_dim] (f32 or bf16, rows may be strided) into the cache's slots [n] int32."""
+    n = slots.shape[0]
+    shape = (n, cache.n_kv, cache.head_dim)
+    if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
+        raise ValueError(f"k and v must be {shape} of one type")
+    hd = cache.head_dim
+    for t in (k, v):
+        if t.stride(2) != 1 or (t.stride(1) != hd and cache.n_kv > 1):
+            raise ValueError("k and v rows must be contiguous")
+    row = cache.n_kv * hd
+    (kp, ks), (vp, vs) = _rows(k, row, "k"), _rows(v, row, "v")
+    check(lib().llama_kv_append_mx(_stream(), cache.ptr, n, _i32(slots, "slots"), _dtype(k), kp, ks, vp, vs))
+
+
+def kv_read_mx(cache: MxKvCache, slots, dtype=torch.bfloat16):
+    """The cached rows in slots [n] int32 as K, V [n][n_kv][head_dim] of `dtype`; zeros for negative slots."""
+    n = slots.shape[0]
+    k = torch.empty((n, cache.n_kv, cache.head_dim), dtype=dtype, device=cache.k.device)
+    v = torch.empty_like(k)
+    check(lib().llama_kv_read_mx(_stream(), cache.ptr, n, _i32(slots, "slots"), _dtype(k), k.data_ptr(), v.data_ptr()))
+    return k, v
+
+
+def attn_mx_workspace(cache: MxKvCache, batch, n_heads, q_len, prefix_len, max_len):
+    """Workspace of attn_paged_mx (prefix_len 0) and attn_shared_mx for this shape."""
+    nbytes = lib().llama_attn_mx_workspace_size(cache.ptr, batch, n_heads, q_len, prefix_len, max_len)
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=cache.k.device)
+
+
+def _attn_args(cache, q, page_table, lens, max_len):
+    if q.dim() != 4 or q.shape[3] != cache.head_dim:
+        raise ValueError(f"q must be [batch][q_len][n_heads][{cache.head_dim}]")
+    B, T, H, hd = q.shape
+    if not q.is_cuda:
+        raise ValueError("fp4x operators take CUDA tensors (no CPU fallback)")
+    sb, st, sh, sd = q.stride()
+    row = st if T > 1 else sb if B > 1 else H * hd
+    if sd != 1 or (sh != hd and H > 1) or (B > 1 and sb != T * row):
+        raise ValueError("q token rows must be contiguous and evenly spaced")
+    if page_table.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,):
+        raise ValueError("page_table must be [batch][pages] and lens [batch]")
+    if max_len is None:
+        max_len = page_table.shape[1] * cache.page_size
+    return B, T, H, row, max_len
+
+
+def attn_paged_mx(cache: MxKvCache, q, page_table, lens, max_len=None, workspace=None):
+    """Attention of q [batch][q_len][n_heads][hd] over each sequence's own pages; lens [batch] int32 counts the cached
+    positions with the q_len new ones as the last.  Returns a tensor shaped like q."""
+    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len)
+    ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, 0, max_len)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    check(lib().llama_attn_paged_mx(_stream(), cache.ptr, B, H, T, _i32(page_table, "page_table"), page_table.shape[1],
+                                    _i32(lens, "lens"), max_len, _dtype(q), q.data_ptr(), row, out.data_ptr(),
+                                    ws.data_ptr(), ws.numel()))
+    return out
+
+
+def attn_shared_mx(cache: MxKvCache, q, prefix_pages, prefix_len, page_table, lens, max_len=None, workspace=None):
+    """attn_paged_mx for sequences that continue one prefix of prefix_len positions behind prefix_pages int32."""
+    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len)
+    if prefix_pages.numel() * cache.page_size < prefix_len:
+        raise ValueError("prefix_pages hold fewer than prefix_len positions")
+    ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, prefix_len, max_len)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    check(lib().llama_attn_shared_mx(_stream(), cache.ptr, B, H, T, _i32(prefix_pages, "prefix_pages"), prefix_len,
+                                     _i32(page_table, "page_table"), page_table.shape[1], _i32(lens, "lens"), max_len,
+                                     _dtype(q), q.data_ptr(), row, out.data_ptr(), ws.data_ptr(), ws.numel()))
+    return out
+
+
+def verify_drafts(logits, drafts, uniforms, noise, draft_probs=None, draft_lens=None, temperature=None,
+                  workspace=None):
+    """Speculative verification: logits [batch][k+1][vocab] (f32 or bf16) of the target, drafts [batch][k] int32,
+    uniforms [batch][k], noise [batch][vocab] exponential draws, draft_probs [batch][k][vocab] (None: certain drafts),
+    draft_lens [batch] int32, temperature [batch].  Returns (accepted [batch] int32, tokens [batch][k+1] int32,
+    logprobs [batch][k+1])."""
+    B, K1, V = logits.shape
+    k = K1 - 1
+    if drafts.shape != (B, k) or uniforms.shape != (B, k) or noise.shape != (B, V):
+        raise ValueError("verify_drafts: drafts, uniforms and noise disagree with the logits' shape")
+    if draft_probs is not None and draft_probs.shape != (B, k, V):
+        raise ValueError("verify_drafts: draft_probs must be [batch][k][vocab]")
+    if (draft_lens is not None and draft_lens.shape != (B,)) or (temperature is not None and temperature.shape != (B,)):
+        raise ValueError("verify_drafts: draft_lens and temperature must be [batch]")
+    stride = logits.stride(1) if K1 > 1 else logits.stride(0) if B > 1 else V
+    if not logits.is_cuda or logits.stride(2) != 1 or (B > 1 and logits.stride(0) != K1 * stride):
+        raise ValueError("verify_drafts: logits must be CUDA rows, evenly spaced")
+    dev = logits.device
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    tokens = torch.empty((B, K1), dtype=torch.int32, device=dev)
+    logprobs = torch.empty((B, K1), dtype=torch.float32, device=dev)
+    if workspace is None:
+        workspace = torch.empty(max(lib().llama_verify_workspace_size(B, k, V), 16), dtype=torch.uint8, device=dev)
+    check(lib().llama_verify_drafts(
+        _stream(), B, k, V, _dtype(logits), logits.data_ptr(), stride,
+        None if draft_probs is None else _f32(draft_probs, "draft_probs"), _i32(drafts, "drafts"),
+        None if draft_lens is None else _i32(draft_lens, "draft_lens"), _f32(uniforms, "uniforms"),
+        _f32(noise, "noise"), None if temperature is None else _f32(temperature, "temperature"), accepted.data_ptr(),
+        tokens.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), workspace.numel()))
+    return accepted, tokens, logprobs
