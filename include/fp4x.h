@@ -277,8 +277,8 @@ FP4X_API size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t ba
  * gives zeros.  page_table [batch] rows of table_stride page ids, at least
  * ceil(max_len / page_size) each; ids outside the cache are not read: their
  * positions are masked and the device error word is set.  Softmax scale
- * 1/sqrt(head_dim), statistics and sums in f32; with bf16 q the probabilities enter
- * the tensor cores as f16, with f32 q both operands as f16 pairs (22 bits).
+ * 1/sqrt(head_dim), statistics and sums in f32; the probabilities enter the tensor
+ * cores with 16 bits (bf16 q) or 24 bits (f32 q, which itself enters with 22).
  * n_heads a multiple of n_kv_heads. */
 FP4X_API int llama_attn_paged_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
                                  uint32_t q_len, const int32_t *page_table, uint32_t table_stride,
