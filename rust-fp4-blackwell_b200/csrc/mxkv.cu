@@ -54,81 +54,150 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// Nearest E2M1 level, ties to the smaller magnitude; v < 0 sets the sign even when it rounds to 0.
-__device__ __forceinline__ uint32_t e2m1_code(float v) {
-    const float a = fabsf(v);
-    const uint32_t c = (a > 0.25f) + (a > 0.75f) + (a > 1.25f) + (a > 1.75f) + (a > 2.5f) + (a > 3.5f) + (a > 5.0f);
-    return c | (v < 0.0f ? 8u : 0u);
+// Two scaled values -> E2M1 codes: nearest level, ties to the smaller magnitude, -0 as
+// +0.  The conversion rounds ties to even; every tie has at most two mantissa bits, so
+// one unit less in the last place turns ties (and exact levels, harmlessly) downwards.
+__device__ __forceinline__ float below_tie(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return __uint_as_float((u << 1) == 0 ? 0u : (u & 0x1FFFFFu) ? u : u - 1);
+}
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
+        : "=r"(r)
+        : "f"(below_tie(hi)), "f"(below_tie(lo)));
+    return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, float (&x)[4]);
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]);
 template <>
-__device__ __forceinline__ void load4<float>(const float *p, float (&x)[4]) {
-    const float4 f = __ldg(reinterpret_cast<const float4 *>(p));
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+__device__ __forceinline__ void load8<float>(const float *p, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 template <>
-__device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[4]) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
-    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[8]) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
 }
 
-// One thread: dimensions 4g..4g+3 of one 32-block; eight neighbouring lanes share the block.
+// Both kernels: four threads share a (K or V, token, head) row; thread t holds chunks
+// 2t and 2t + 1, dimensions 8t..8t+7 of every 32-block, so it moves 16-byte pieces on
+// both sides and a block's maximum takes two shuffles.  Bound by HBM.
+template <uint32_t HD>
+struct RowId {
+    uint32_t t, head, is_v, token;
+    __device__ __forceinline__ RowId(uint64_t i, uint32_t n_kv) {
+        t = (uint32_t)(i & 3);
+        const uint64_t r = i >> 2;
+        const uint64_t tk = r / n_kv;
+        head = (uint32_t)(r - tk * n_kv), is_v = (uint32_t)(tk & 1), token = (uint32_t)(tk >> 1);
+    }
+};
+
+template <uint32_t WORDS>
+__device__ __forceinline__ void store_words(uint8_t *p, const uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < WORDS; i += 4)
+            reinterpret_cast<uint4 *>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    }
+}
+template <uint32_t WORDS>
+__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[WORDS]) {
+    if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < WORDS; i += 4) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p) + i / 4);
+            w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+        }
+    } else {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = u.x, w[1] = u.y;
+    }
+}
+
 template <uint32_t FMT, uint32_t HD, typename T>
 __global__ void __launch_bounds__(256) kv_append_kernel(Cache c, uint32_t n, const int32_t *__restrict__ slots,
                                                         const T *__restrict__ k, uint64_t ks, const T *__restrict__ v,
                                                         uint64_t vs) {
-    constexpr uint32_t NB = HD / 32;
-    const uint64_t per = (uint64_t)c.n_kv * NB * 8, total = (uint64_t)n * 2 * per;
+    constexpr uint32_t NB = HD / 32, WORDS = Row<FMT, HD>::CHUNK / 2;
     const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= total) return;  // whole groups of 8 lanes: per is a multiple of 8
-    const uint32_t g = (uint32_t)(i & 7), b = (uint32_t)(i >> 3) % NB;
-    const uint64_t r = i / (8 * NB);
-    const uint32_t head = (uint32_t)(r % c.n_kv);
-    const uint32_t is_v = (uint32_t)((r / c.n_kv) & 1);
-    const uint32_t tok = (uint32_t)(r / c.n_kv / 2);
-    float x[4];
-    load4<T>((is_v ? v + tok * vs : k + tok * ks) + head * HD + b * 32 + g * 4, x);
-    float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    uint32_t nan = (x[0] != x[0]) | (x[1] != x[1]) | (x[2] != x[2]) | (x[3] != x[3]);
-    const uint32_t mask = 0xFFu << (threadIdx.x & 24);
+    if (i >= (uint64_t)n * 2 * c.n_kv * 4) return;  // whole rows of four lanes
+    const RowId<HD> id(i, c.n_kv);
+    const int32_t slot = slots[id.token];
+    const T *src = (id.is_v ? v + id.token * vs : k + id.token * ks) + id.head * HD + id.t * 8;
+    float x[NB][8];
 #pragma unroll
-    for (int o = 1; o < 8; o *= 2) {
-        amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-        nan |= __shfl_xor_sync(mask, nan, o);
+    for (uint32_t b = 0; b < NB; ++b) load8<T>(src + b * 32, x[b]);
+    const uint32_t mask = 0xFu << (threadIdx.x & 28);
+    uint32_t w[WORDS], scales = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < WORDS; ++j) w[j] = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        float amax = 0.0f;
+        uint32_t nan = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            amax = fmaxf(amax, fabsf(x[b][j]));
+            if (FMT == FMT_FP4) nan |= x[b][j] != x[b][j];
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 2));
+        uint32_t e = e8m0_of(amax, FMT == FMT_FP8 ? 8 : 2);
+        float s0, s1;
+        inv_scale(e, s0, s1);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) x[b][j] = x[b][j] * s0 * s1;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {  // chunk 2t + h: its four codes of block b at position 4 b
+            const float *y = x[b] + 4 * h;
+            if constexpr (FMT == FMT_FP8) {
+                w[h * NB + b] = e4m3x2(y[0], y[1]) | (e4m3x2(y[2], y[3]) << 16);
+            } else {
+                const uint32_t half = e2m1x2(y[0], y[1]) | (e2m1x2(y[2], y[3]) << 8);
+                w[(h * NB + b) / 2] |= half << (16 * (b & 1));
+            }
+        }
+        if (FMT == FMT_FP4 && __any_sync(mask, nan)) e = 255;
+        scales |= e << (8 * b);
     }
-    uint32_t e = e8m0_of(amax, FMT == FMT_FP8 ? 8 : 2);
-    float s0, s1;
-    inv_scale(e, s0, s1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = x[j] * s0 * s1;
-    const int32_t slot = slots[tok];
     if (slot < 0) return;
     const uint32_t page = (uint32_t)slot >> c.page_shift, row = (uint32_t)slot & ((1u << c.page_shift) - 1);
     if (page >= c.n_pages) {
         raise_device_error(DEVERR_BAD_ARG);
         return;
     }
-    uint8_t *dst = (is_v ? c.v : c.k) + code_off<FMT, HD>(c, page, head, row);
-    if (FMT == FMT_FP8) {
-        *reinterpret_cast<uint32_t *>(dst + (g * NB + b) * 4) = e4m3x2(x[0], x[1]) | (e4m3x2(x[2], x[3]) << 16);
-    } else {
-        *reinterpret_cast<uint16_t *>(dst + (g * NB + b) * 2) =
-            (uint16_t)(e2m1_code(x[0]) | (e2m1_code(x[1]) << 4) | (e2m1_code(x[2]) << 8) | (e2m1_code(x[3]) << 12));
-        if (nan) e = 255;
+    store_words<WORDS>((id.is_v ? c.v : c.k) + code_off<FMT, HD>(c, page, id.head, row) + id.t * WORDS * 4, w);
+    if (id.t == 0) {
+        uint8_t *dst = (id.is_v ? c.vs : c.ks) + scale_off<HD>(c, page, id.head, row);
+        if (NB == 4)
+            *reinterpret_cast<uint32_t *>(dst) = scales;
+        else
+            *reinterpret_cast<uint16_t *>(dst) = (uint16_t)scales;
     }
-    if (g == 0) ((is_v ? c.vs : c.ks) + scale_off<HD>(c, page, head, row))[b] = (uint8_t)e;
 }
 
 // ---------------------------------------------------------------- read
-__device__ __forceinline__ void store4(float *p, const float (&x)[4]) {
-    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
-__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float (&x)[4]) {
-    __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<uint32_t *>(&a), *reinterpret_cast<uint32_t *>(&b));
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
@@ -140,38 +209,46 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
 template <uint32_t FMT, uint32_t HD, typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(Cache c, uint32_t n, const int32_t *__restrict__ slots,
                                                       T *__restrict__ k, T *__restrict__ v) {
-    constexpr uint32_t NB = HD / 32;
-    const uint64_t per = (uint64_t)c.n_kv * NB * 8, total = (uint64_t)n * 2 * per;
+    constexpr uint32_t NB = HD / 32, WORDS = Row<FMT, HD>::CHUNK / 2;
     const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= total) return;
-    const uint32_t g = (uint32_t)(i & 7), b = (uint32_t)(i >> 3) % NB;
-    const uint64_t r = i / (8 * NB);
-    const uint32_t head = (uint32_t)(r % c.n_kv);
-    const uint32_t is_v = (uint32_t)((r / c.n_kv) & 1);
-    const uint32_t tok = (uint32_t)(r / c.n_kv / 2);
-    const int32_t slot = slots[tok];
+    if (i >= (uint64_t)n * 2 * c.n_kv * 4) return;
+    const RowId<HD> id(i, c.n_kv);
+    const int32_t slot = slots[id.token];
     const uint32_t page = (uint32_t)slot >> c.page_shift, row = (uint32_t)slot & ((1u << c.page_shift) - 1);
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t w[WORDS], scales = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < WORDS; ++j) w[j] = 0;
     if (slot >= 0 && page < c.n_pages) {
-        const uint8_t *src = (is_v ? c.v : c.k) + code_off<FMT, HD>(c, page, head, row);
-        const float s = e8m0_to_f32(((is_v ? c.vs : c.ks) + scale_off<HD>(c, page, head, row))[b]);
-        uint32_t h[2];
-        if (FMT == FMT_FP8) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(src + (g * NB + b) * 4);
-            h[0] = e4m3x2_to_f16x2(w & 0xFFFFu), h[1] = e4m3x2_to_f16x2(w >> 16);
-        } else {
-            const uint32_t w = *reinterpret_cast<const uint16_t *>(src + (g * NB + b) * 2);
-            h[0] = e2m1x2_to_f16x2(w & 0xFFu), h[1] = e2m1x2_to_f16x2(w >> 8);
-        }
-        const float2 lo = __half22float2(*reinterpret_cast<__half2 *>(&h[0]));
-        const float2 hi = __half22float2(*reinterpret_cast<__half2 *>(&h[1]));
-        x[0] = lo.x * s, x[1] = lo.y * s, x[2] = hi.x * s, x[3] = hi.y * s;
+        load_words<WORDS>((id.is_v ? c.v : c.k) + code_off<FMT, HD>(c, page, id.head, row) + id.t * WORDS * 4, w);
+        const uint8_t *src = (id.is_v ? c.vs : c.ks) + scale_off<HD>(c, page, id.head, row);
+        scales = NB == 4 ? *reinterpret_cast<const uint32_t *>(src) : *reinterpret_cast<const uint16_t *>(src);
     } else if (slot >= 0) {
         raise_device_error(DEVERR_BAD_ARG);
     }
-    store4((is_v ? v : k) + ((uint64_t)tok * c.n_kv + head) * HD + b * 32 + g * 4, x);
+    T *dst = (id.is_v ? v : k) + ((uint64_t)id.token * c.n_kv + id.head) * HD + id.t * 8;
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        const float s = e8m0_to_f32((scales >> (8 * b)) & 0xFF);
+        float x[8];
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            uint32_t f[2];
+            if constexpr (FMT == FMT_FP8) {
+                const uint32_t y = w[h * NB + b];
+                f[0] = e4m3x2_to_f16x2(y & 0xFFFFu), f[1] = e4m3x2_to_f16x2(y >> 16);
+            } else {
+                const uint32_t y = w[(h * NB + b) / 2] >> (16 * (b & 1));
+                f[0] = e2m1x2_to_f16x2(y & 0xFF), f[1] = e2m1x2_to_f16x2((y >> 8) & 0xFF);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                const float2 z = __half22float2(*reinterpret_cast<const __half2 *>(&f[j]));
+                x[4 * h + 2 * j] = z.x * s, x[4 * h + 2 * j + 1] = z.y * s;
+            }
+        }
+        store8(dst + b * 32, x);
+    }
 }
-
 
 }  // namespace mxkv
 }  // namespace fp4x
@@ -191,7 +268,7 @@ extern "C" int llama_kv_append_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, 
                  "llama_kv_append_mx: rows of k and v must be 16-byte aligned");
     FP4X_REQUIRE(k_stride >= (uint64_t)c.n_kv * hd && v_stride >= (uint64_t)c.n_kv * hd,
                  "llama_kv_append_mx: row stride below n_kv_heads * head_dim");
-    const uint64_t blocks = ((uint64_t)n * 2 * c.n_kv * (hd / 4) + 255) / 256;
+    const uint64_t blocks = ((uint64_t)n * 2 * c.n_kv * 4 + 255) / 256;
     FP4X_REQUIRE(blocks <= 0x7FFFFFFFull, "llama_kv_append_mx: too many rows");
     cudaStream_t st = (cudaStream_t)stream;
 #define FP4X_LAUNCH(FMT, HD, T)                                                                             \
@@ -220,7 +297,7 @@ extern "C" int llama_kv_read_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, ui
     FP4X_REQUIRE(mxkv::aligned(k_out, 16) && mxkv::aligned(v_out, 16),
                  "llama_kv_read_mx: outputs must be 16-byte aligned");
     const uint32_t hd = cache->head_dim;
-    const uint64_t blocks = ((uint64_t)n * 2 * c.n_kv * (hd / 4) + 255) / 256;
+    const uint64_t blocks = ((uint64_t)n * 2 * c.n_kv * 4 + 255) / 256;
     FP4X_REQUIRE(blocks <= 0x7FFFFFFFull, "llama_kv_read_mx: too many rows");
     cudaStream_t st = (cudaStream_t)stream;
 #define FP4X_LAUNCH(FMT, HD, T) \

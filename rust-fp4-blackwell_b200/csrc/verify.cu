@@ -6,13 +6,31 @@
 // max(p - q, 0), a fully accepted draft from p_k.  Sampling by an exponential race:
 // argmax_v w(v) / E(v) with E ~ Exp(1) picks v with probability w(v) / sum w, needs
 // no normalised or running sums, and so does not hang on the order of a sum.
-#include "common.cuh"
+//
+// Two kernels.  verify_stats_kernel reads every target row once (bound by HBM): each
+// CTA takes a slice of one row and leaves (maximum, its index, sum of exp(x - max)).
+// verify_choose_kernel, a cluster of eight CTAs per sequence, joins the slices, walks
+// the drafts, and runs the race over the one row that decides; the row was read
+// moments before, so most of it comes from L2.
+#include <cooperative_groups.h>
+
+#include "mxkv.cuh"
 
 namespace fp4x {
 namespace verify {
 
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kCluster = 8;
+constexpr uint32_t kMaxSlices = 32;  // slices of a row: one lane each when they are joined
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Stat {  // of a slice or row: max logit, sum of exp((x - max) / T), lowest index of the max
+    float m, s;
+    uint32_t i, pad;
+};
+
 struct Params {
-    uint32_t batch, k, vocab;
+    uint32_t batch, k, vocab, slices;
     const void *logits;
     uint64_t stride;
     const float *probs;
@@ -20,103 +38,288 @@ struct Params {
     const float *u, *noise, *temp;
     int32_t *accepted, *tokens;
     float *logprobs;
+    Stat *stats;  // [batch * (k + 1)][slices]
 };
 
-__device__ __forceinline__ float clean(float x) {  // NaN -> -inf, +inf -> the largest finite value
-    return x != x ? -INFINITY : fminf(x, 3.40282347e+38f);
+// NaN -> -inf (fmaxf returns the other operand), +inf -> the largest finite value.
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 3.40282347e+38f); }
+
+// Four consecutive values: one 16- or 8-byte load where rows are aligned for it
+// (VEC), else single loads.
+template <bool VEC>
+__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
+    if constexpr (VEC) {
+        const float4 f = __ldg(reinterpret_cast<const float4 *>(p));
+        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __ldg(p + i);
+    }
 }
-__device__ __forceinline__ float as_f32(float x) { return x; }
-__device__ __forceinline__ float as_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <bool VEC>
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float (&x)[4]) {
+    if constexpr (VEC) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+        x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
+        x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+    }
+}
+__device__ __forceinline__ float load1(const float *p) { return *p; }
+__device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+
+__device__ __forceinline__ uint32_t drafts_of(const Params &p, uint32_t b) {
+    return p.lens ? (uint32_t)min(max(p.lens[b], 0), (int32_t)p.k) : p.k;
+}
+// log2(e) / T, or log2(e) for greedy sequences (their log-probabilities are at T = 1).
+__device__ __forceinline__ float factor_of(const Params &p, uint32_t b, bool &greedy) {
+    const float t = p.temp ? p.temp[b] : 1.0f;
+    greedy = !(t > 1e-30f);
+    return greedy ? kLog2e : kLog2e / t;
+}
+
+__device__ __forceinline__ Stat join(const Stat &a, const Stat &b, float c) {
+    Stat r;
+    r.m = fmaxf(a.m, b.m);
+    r.i = a.m > b.m || (a.m == b.m && a.i < b.i) ? a.i : b.i;
+    r.s = r.m == -INFINITY ? 0.0f : a.s * exp2f((a.m - r.m) * c) + b.s * exp2f((b.m - r.m) * c);
+    r.pad = 0;
+    return r;
+}
+__device__ __forceinline__ Stat warp_join(Stat x, float c) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Stat y;
+        y.m = __shfl_xor_sync(~0u, x.m, o), y.s = __shfl_xor_sync(~0u, x.s, o), y.i = __shfl_xor_sync(~0u, x.i, o);
+        x = join(x, y, c);
+    }
+    return x;
+}
+
+// Slice of a row in units of four values.
+__device__ __forceinline__ void slice_of(uint32_t vocab, uint32_t n, uint32_t s, uint32_t &lo, uint32_t &hi) {
+    const uint32_t quads = (vocab + 3) / 4;
+    lo = (uint32_t)((uint64_t)s * quads / n) * 4;
+    hi = min(vocab, (uint32_t)((uint64_t)(s + 1) * quads / n) * 4);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_constant__ Params p) {
+    __shared__ Stat part[kThreads / 32];
+    const uint32_t row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+    const uint32_t b = row / (p.k + 1), i = row % (p.k + 1);
+    if (i > drafts_of(p, b)) return;
+    bool greedy;
+    const float c = factor_of(p, b, greedy);
+    uint32_t lo, hi;
+    slice_of(p.vocab, p.slices, slice, lo, hi);
+    const T *x = (const T *)p.logits + (uint64_t)row * p.stride;
+    Stat st{-INFINITY, 0.0f, 0xFFFFFFFFu, 0};
+    constexpr uint32_t U = 4;  // loads in flight per thread
+    for (uint32_t v0 = lo + threadIdx.x * 4; v0 < hi; v0 += kThreads * 4 * U) {
+        float y[U][4];
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j) {
+            const uint32_t v = v0 + j * kThreads * 4;
+            if (v + 4 <= hi) {
+                load4<VEC>(x + v, y[j]);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) y[j][e] = v + e < hi ? load1(x + v + e) : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) y[j][e] = clean(y[j][e]), mx = fmaxf(mx, y[j][e]);
+        if (mx > st.m) {
+            st.s = st.s * exp2f((st.m - mx) * c), st.m = mx;
+            uint32_t at = 0;  // lowest index that holds the maximum: j ascending, then e
+#pragma unroll
+            for (int j = U - 1; j >= 0; --j)
+#pragma unroll
+                for (int e = 3; e >= 0; --e)
+                    if (y[j][e] == mx) at = v0 + j * kThreads * 4 + e;
+            st.i = at;
+        }
+        if (st.m > -INFINITY) {
+            float s = 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) s += exp2f((y[j][e] - st.m) * c);
+            st.s += s;
+        }
+    }
+    st = warp_join(st, c);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = st;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        st = threadIdx.x < kThreads / 32 ? part[threadIdx.x] : Stat{-INFINITY, 0.0f, 0xFFFFFFFFu, 0};
+        st = warp_join(st, c);
+        if (threadIdx.x == 0) p.stats[(uint64_t)row * p.slices + slice] = st;
+    }
+}
 
 struct Best {
     float v;
     uint32_t i;
 };
 __device__ __forceinline__ Best better(Best a, Best b) { return b.v > a.v || (b.v == a.v && b.i < a.i) ? b : a; }
-
-__device__ Best block_best(Best x, Best *buf) {
+__device__ __forceinline__ Best warp_best(Best x) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         x = better(x, Best{__shfl_xor_sync(~0u, x.v, o), __shfl_xor_sync(~0u, x.i, o)});
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = x;
-    __syncthreads();
-    x = buf[0];
-    for (uint32_t w = 1; w < blockDim.x / 32; ++w) x = better(x, buf[w]);
     return x;
 }
 
-// One CTA per sequence walks its rows.
-template <typename T>
-__global__ void __launch_bounds__(512) verify_kernel(Params p) {
-    __shared__ Best buf[16];
-    __shared__ float sums[16];
-    const uint32_t b = blockIdx.x;
-    const uint32_t n_draft = p.lens ? (uint32_t)min(max(p.lens[b], 0), (int32_t)p.k) : p.k;
-    const float t = p.temp ? p.temp[b] : 1.0f;
-    const bool greedy = !(t > 1e-30f);
-    const float inv_t = greedy ? 1.0f : t;
-    for (uint32_t i = 0;; ++i) {
-        const T *x = (const T *)p.logits + ((uint64_t)b * (p.k + 1) + i) * p.stride;
-        Best top{-INFINITY, 0xFFFFFFFFu};
-        for (uint32_t v = threadIdx.x; v < p.vocab; v += blockDim.x) top = better(top, Best{clean(as_f32(x[v])), v});
-        top = block_best(top, buf);
-        if (top.v == -INFINITY) top.i = 0;
-        float s = 0.0f;
-        for (uint32_t v = threadIdx.x; v < p.vocab; v += blockDim.x) {
-            const float y = clean(as_f32(x[v]));
-            if (y > -INFINITY) s += expf((y - top.v) / inv_t);
-        }
-        s = warp_sum(s);
-        __syncthreads();
-        if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = s;
-        __syncthreads();
-        s = 0.0f;
-        for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += sums[w];
-        const float *q = p.probs ? p.probs + ((uint64_t)b * p.k + i) * p.vocab : nullptr;
-        int32_t tok;
-        bool ok = false;
-        if (i < n_draft) {
-            tok = p.drafts[b * p.k + i];
-            if ((uint32_t)tok < p.vocab) {
-                const float y = clean(as_f32(x[tok]));
-                const float pd = y > -INFINITY ? expf((y - top.v) / inv_t) / s : 0.0f;
-                ok = greedy ? (uint32_t)tok == top.i : p.u[b * p.k + i] * (q ? q[tok] : 1.0f) < pd;
-            }
-        }
-        if (!ok) {
-            const bool residual = i < n_draft;
-            const uint32_t d = (uint32_t)tok;
-            if (greedy) {
-                tok = (int32_t)top.i;
-            } else {
-                for (int pass = residual ? 0 : 1; pass < 2; ++pass) {
-                    Best best{0.0f, 0xFFFFFFFFu};
-                    for (uint32_t v = threadIdx.x; v < p.vocab; v += blockDim.x) {
-                        const float y = clean(as_f32(x[v]));
-                        float w = y > -INFINITY ? expf((y - top.v) / inv_t) / s : 0.0f;
-                        if (pass == 0) w = fmaxf(w - (q ? q[v] : v == d ? 1.0f : 0.0f), 0.0f);
-                        if (w > 0.0f) best = better(best, Best{w / p.noise[(uint64_t)b * p.vocab + v], v});
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
+    verify_choose_kernel(const __grid_constant__ Params p) {
+    namespace cg = cooperative_groups;
+    constexpr uint32_t W = kThreads / 32;
+    __shared__ Stat rows[256];  // k + 1 <= 256
+    __shared__ float pd[256];   // p_i(d_i) / q_i(d_i) test as 0 / 1
+    __shared__ Best part[2][W], mine[2];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t b = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t n_draft = drafts_of(p, b);
+    bool greedy;
+    const float c = factor_of(p, b, greedy);
+    pdl_wait();
+    const uint64_t first = (uint64_t)b * (p.k + 1);
+    // ---- join the slices of every row, test the drafts
+    for (uint32_t i = warp; i <= n_draft; i += W) {
+        Stat st = lane < p.slices ? p.stats[(first + i) * p.slices + lane] : Stat{-INFINITY, 0.0f, 0xFFFFFFFFu, 0};
+        st = warp_join(st, c);
+        if (st.m == -INFINITY) st.i = 0;
+        if (lane == 0) {
+            rows[i] = st;
+            bool ok = false;
+            if (i < n_draft) {
+                const int32_t d = p.drafts[(uint64_t)b * p.k + i];
+                if ((uint32_t)d < p.vocab) {
+                    if (greedy) {
+                        ok = (uint32_t)d == st.i;
+                    } else {
+                        const float y = clean(load1((const T *)p.logits + (first + i) * p.stride + d));
+                        const float pr = y > -INFINITY ? exp2f((y - st.m) * c) / st.s : 0.0f;
+                        const float qr = p.probs ? p.probs[((uint64_t)b * p.k + i) * p.vocab + d] : 1.0f;
+                        ok = p.u[(uint64_t)b * p.k + i] * qr < pr;
                     }
-                    best = block_best(best, buf);
-                    tok = (int32_t)(best.i == 0xFFFFFFFFu ? top.i : best.i);
-                    if (best.i != 0xFFFFFFFFu) break;
                 }
             }
-        }
-        if (threadIdx.x == 0) {
-            p.tokens[b * (p.k + 1) + i] = tok;
-            if (p.logprobs) p.logprobs[b * (p.k + 1) + i] = s > 0.0f ? (clean(as_f32(x[tok])) - top.v) / inv_t - logf(s) : -INFINITY;
-        }
-        if (!ok) {
-            if (threadIdx.x == 0) p.accepted[b] = (int32_t)i;
-            for (uint32_t j = i + 1 + threadIdx.x; j <= p.k; j += blockDim.x) {
-                p.tokens[b * (p.k + 1) + j] = -1;
-                if (p.logprobs) p.logprobs[b * (p.k + 1) + j] = 0.0f;
-            }
-            return;
+            pd[i] = ok ? 1.0f : 0.0f;
         }
     }
+    __syncthreads();
+    uint32_t at = 0;
+    while (at < n_draft && pd[at] != 0.0f) ++at;
+    const Stat st = rows[at];
+    const T *x = (const T *)p.logits + (first + at) * p.stride;
+    // ---- the race: over max(p - q, 0), and over p should that leave nothing
+    Best best[2] = {{0.0f, 0xFFFFFFFFu}, {0.0f, 0xFFFFFFFFu}};
+    if (!greedy && st.m > -INFINITY) {
+        const bool rejected = at < n_draft;
+        const float *q = rejected && p.probs ? p.probs + ((uint64_t)b * p.k + at) * p.vocab : nullptr;
+        const uint32_t d = rejected && !p.probs ? (uint32_t)p.drafts[(uint64_t)b * p.k + at] : 0xFFFFFFFFu;
+        const float *noise = p.noise + (uint64_t)b * p.vocab;
+        const float inv = 1.0f / st.s;
+        uint32_t lo, hi;
+        slice_of(p.vocab, kCluster, rank, lo, hi);
+        constexpr uint32_t U = 2;
+        for (uint32_t v0 = lo + threadIdx.x * 4; v0 < hi; v0 += kThreads * 4 * U) {
+            float y[U][4], qv[U][4], ev[U][4];
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j) {
+                const uint32_t v = v0 + j * kThreads * 4;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) y[j][e] = -INFINITY, qv[j][e] = 0.0f, ev[j][e] = 1.0f;
+                if (v + 4 <= hi) {
+                    load4<VEC>(x + v, y[j]);
+                    load4<VEC>(noise + v, ev[j]);
+                    if (q) load4<VEC>(q + v, qv[j]);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e)
+                        if (v + e < hi) {
+                            y[j][e] = load1(x + v + e), ev[j][e] = noise[v + e];
+                            if (q) qv[j][e] = q[v + e];
+                        }
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < U; ++j)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const uint32_t v = v0 + j * kThreads * 4 + e;
+                    const float w = exp2f((clean(y[j][e]) - st.m) * c) * inv;
+                    const float r = v == d ? 0.0f : fmaxf(w - qv[j][e], 0.0f);  // certain drafts: q = 1 at d
+                    const float f = __fdividef(1.0f, ev[j][e]);
+                    // indices ascend within a thread: a strict comparison keeps the lowest
+                    if (r > 0.0f && r * f > best[0].v) best[0] = Best{r * f, v};
+                    if (w > 0.0f && w * f > best[1].v) best[1] = Best{w * f, v};
+                }
+        }
+    }
+#pragma unroll
+    for (uint32_t z = 0; z < 2; ++z) {
+        best[z] = warp_best(best[z]);
+        if (lane == 0) part[z][warp] = best[z];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        Best r = part[threadIdx.x][0];
+        for (uint32_t w = 1; w < W; ++w) r = better(r, part[threadIdx.x][w]);
+        mine[threadIdx.x] = r;
+    }
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+        Best r[2];
+#pragma unroll
+        for (uint32_t z = 0; z < 2; ++z)
+            r[z] = warp_best(lane < kCluster ? *cluster.map_shared_rank(&mine[z], lane) : Best{0.0f, 0xFFFFFFFFu});
+        const uint32_t pick = r[0].i != 0xFFFFFFFFu ? r[0].i : r[1].i != 0xFFFFFFFFu ? r[1].i : st.i;
+        const uint64_t out = (uint64_t)b * (p.k + 1);
+        for (uint32_t i = lane; i <= p.k; i += 32) {
+            const int32_t tok = i < at ? p.drafts[(uint64_t)b * p.k + i] : i == at ? (int32_t)pick : -1;
+            p.tokens[out + i] = tok;
+            if (p.logprobs) {
+                float lp = 0.0f;
+                if (i <= at) {
+                    const Stat ri = rows[i];
+                    const float y = clean(load1((const T *)p.logits + (first + i) * p.stride + tok));
+                    lp = ri.s > 0.0f ? (y - ri.m) * c * 0.6931471805599453f - logf(ri.s) : -INFINITY;
+                }
+                p.logprobs[out + i] = lp;
+            }
+        }
+        if (lane == 0) p.accepted[b] = (int32_t)at;
+    }
+    cluster.sync();  // no CTA leaves while its shared memory may be read
+}
+
+// Slices per row: enough CTAs for two waves of the 2048-thread SMs, and no slice below
+// 2048 values (its join would cost as much as its reading).
+inline uint32_t slices_of(uint64_t rows, uint32_t vocab) {
+    const uint64_t want = (uint64_t)num_sms() * 16 / (rows ? rows : 1), most = vocab / 2048;
+    const uint64_t n = want < most ? want : most;
+    return (uint32_t)(n < 1 ? 1 : n > kMaxSlices ? kMaxSlices : n);
+}
+
+template <typename T, bool VEC>
+int launch(cudaStream_t st, const Params &p) {
+    const uint64_t ctas = (uint64_t)p.batch * (p.k + 1) * p.slices;
+    verify_stats_kernel<T, VEC><<<(uint32_t)ctas, kThreads, 0, st>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess)
+        e = launch_pdl(verify_choose_kernel<T, VEC>, dim3(p.batch * kCluster), dim3(kThreads), 0, st, p);
+    if (e != cudaSuccess) return set_error("llama_verify_drafts: %s", cudaGetErrorString(e)), FP4X_ECUDA;
+    return FP4X_OK;
 }
 
 }  // namespace verify
@@ -124,7 +327,10 @@ __global__ void __launch_bounds__(512) verify_kernel(Params p) {
 
 using namespace fp4x;
 
-extern "C" size_t llama_verify_workspace_size(uint32_t batch, uint32_t k, uint32_t vocab) { return 0; }
+extern "C" size_t llama_verify_workspace_size(uint32_t batch, uint32_t k, uint32_t vocab) {
+    const uint64_t rows = (uint64_t)batch * (k + 1);
+    return (size_t)(rows * verify::slices_of(rows, vocab) * sizeof(verify::Stat));
+}
 
 extern "C" int llama_verify_drafts(fp4x_stream_t stream, uint32_t batch, uint32_t k, uint32_t vocab, uint32_t dtype,
                                    const void *logits, uint64_t logits_stride, const float *draft_probs,
@@ -139,16 +345,20 @@ extern "C" int llama_verify_drafts(fp4x_stream_t stream, uint32_t batch, uint32_
     FP4X_REQUIRE(batch <= 65535, "llama_verify_drafts: batch %u above 65535", batch);
     FP4X_REQUIRE(logits && noise && accepted && tokens && (k == 0 || (drafts && uniforms)),
                  "llama_verify_drafts: null pointer");
-    FP4X_REQUIRE(mxkv::aligned(logits, dtype == FP4X_F32 ? 4 : 2), "llama_verify_drafts: misaligned logits");
+    const uint32_t elem = dtype == FP4X_F32 ? 4 : 2;
+    FP4X_REQUIRE(mxkv::aligned(logits, elem), "llama_verify_drafts: misaligned logits");
     const size_t need = llama_verify_workspace_size(batch, k, vocab);
-    FP4X_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+    FP4X_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need,
                  "llama_verify_drafts: workspace of %zu bytes (16-byte aligned) needed, %zu given", need,
                  workspace_bytes);
-    verify::Params p{batch, k, vocab, logits, logits_stride, draft_probs, drafts, draft_lens, uniforms, noise,
-                     temperature, accepted, tokens, logprobs};
-    if (dtype == FP4X_F32)
-        verify::verify_kernel<float><<<batch, 512, 0, (cudaStream_t)stream>>>(p);
-    else
-        verify::verify_kernel<__nv_bfloat16><<<batch, 512, 0, (cudaStream_t)stream>>>(p);
-    return check_launch("llama_verify_drafts");
+    const uint64_t rows = (uint64_t)batch * (k + 1);
+    verify::Params p{batch, k, vocab, verify::slices_of(rows, vocab), logits, logits_stride, draft_probs, drafts,
+                     draft_lens, uniforms, noise, temperature, accepted, tokens, logprobs,
+                     (verify::Stat *)workspace};
+    // four values per load where every row of every operand starts on a boundary of four
+    const bool vec = vocab % 4 == 0 && logits_stride % 4 == 0 && mxkv::aligned(logits, 4 * elem) &&
+                     aligned16(noise) && aligned16(draft_probs);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == FP4X_F32) return vec ? verify::launch<float, true>(st, p) : verify::launch<float, false>(st, p);
+    return vec ? verify::launch<__nv_bfloat16, true>(st, p) : verify::launch<__nv_bfloat16, false>(st, p);
 }

@@ -11,7 +11,8 @@ from . import MxKv, check, lib
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream of the current device, without building a torch.cuda.Stream (3 us per call)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: torch.Tensor):
@@ -303,8 +304,7 @@ def kv_append_mx(cache: MxKvCache, slots, k, v):
 def kv_read_mx(cache: MxKvCache, slots, dtype=torch.bfloat16):
     """The cached rows in slots [n] int32 as K, V [n][n_kv][head_dim] of `dtype`; zeros for negative slots."""
     n = slots.shape[0]
-    k = torch.empty((n, cache.n_kv, cache.head_dim), dtype=dtype, device=cache.k.device)
-    v = torch.empty_like(k)
+    k, v = cache.k.new_empty((2, n, cache.n_kv, cache.head_dim), dtype=dtype).unbind(0)
     check(lib().llama_kv_read_mx(_stream(), cache.ptr, n, _i32(slots, "slots"), _dtype(k), k.data_ptr(), v.data_ptr()))
     return k, v
 
@@ -312,7 +312,7 @@ def kv_read_mx(cache: MxKvCache, slots, dtype=torch.bfloat16):
 def attn_mx_workspace(cache: MxKvCache, batch, n_heads, q_len, prefix_len, max_len):
     """Workspace of attn_paged_mx (prefix_len 0) and attn_shared_mx for this shape."""
     nbytes = lib().llama_attn_mx_workspace_size(cache.ptr, batch, n_heads, q_len, prefix_len, max_len)
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=cache.k.device)
+    return cache.k.new_empty(max(nbytes, 16))
 
 
 def _attn_args(cache, q, page_table, lens, max_len):
@@ -337,7 +337,7 @@ def attn_paged_mx(cache: MxKvCache, q, page_table, lens, max_len=None, workspace
     positions with the q_len new ones as the last.  Returns a tensor shaped like q."""
     B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len)
     ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, 0, max_len)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     check(lib().llama_attn_paged_mx(_stream(), cache.ptr, B, H, T, _i32(page_table, "page_table"), page_table.shape[1],
                                     _i32(lens, "lens"), max_len, _dtype(q), q.data_ptr(), row, out.data_ptr(),
                                     ws.data_ptr(), ws.numel()))
@@ -350,7 +350,7 @@ def attn_shared_mx(cache: MxKvCache, q, prefix_pages, prefix_len, page_table, le
     if prefix_pages.numel() * cache.page_size < prefix_len:
         raise ValueError("prefix_pages hold fewer than prefix_len positions")
     ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, prefix_len, max_len)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     check(lib().llama_attn_shared_mx(_stream(), cache.ptr, B, H, T, _i32(prefix_pages, "prefix_pages"), prefix_len,
                                      _i32(page_table, "page_table"), page_table.shape[1], _i32(lens, "lens"), max_len,
                                      _dtype(q), q.data_ptr(), row, out.data_ptr(), ws.data_ptr(), ws.numel()))
@@ -374,12 +374,10 @@ def verify_drafts(logits, drafts, uniforms, noise, draft_probs=None, draft_lens=
     stride = logits.stride(1) if K1 > 1 else logits.stride(0) if B > 1 else V
     if not logits.is_cuda or logits.stride(2) != 1 or (B > 1 and logits.stride(0) != K1 * stride):
         raise ValueError("verify_drafts: logits must be CUDA rows, evenly spaced")
-    dev = logits.device
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    tokens = torch.empty((B, K1), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((B, K1), dtype=torch.float32, device=dev)
+    accepted, tokens = drafts.new_empty(B), drafts.new_empty((B, K1))
+    logprobs = uniforms.new_empty((B, K1))
     if workspace is None:
-        workspace = torch.empty(max(lib().llama_verify_workspace_size(B, k, V), 16), dtype=torch.uint8, device=dev)
+        workspace = drafts.new_empty(max(lib().llama_verify_workspace_size(B, k, V), 16), dtype=torch.uint8)
     check(lib().llama_verify_drafts(
         _stream(), B, k, V, _dtype(logits), logits.data_ptr(), stride,
         None if draft_probs is None else _f32(draft_probs, "draft_probs"), _i32(drafts, "drafts"),
