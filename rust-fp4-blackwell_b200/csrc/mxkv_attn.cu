@@ -32,7 +32,7 @@ struct Job {
     uint32_t n_seq, rows, row_tiles, ctas;  // sequences, query rows per (sequence, KV head), tiles of them, grid
     const int32_t *pages, *lens;            // lens null: every sequence holds max_len positions
     uint32_t table_stride, max_len;
-    float *slots;      // 2 per CTA: partial results of segments that CTAs share
+    float *slots;      // 2 per CTA: its part of a segment that began before it, and of one that it began
     float *row_slots;  // one per output row for segments of one CTA (null: written to out)
 };
 
@@ -51,18 +51,25 @@ __device__ __forceinline__ uint32_t seq_len(const Job &j, uint32_t s) {
 }
 __device__ __forceinline__ uint32_t seq_chunks(const Job &j, uint32_t s) { return (seq_len(j, s) + kChunk - 1) / kChunk; }
 
-// The work is every (sequence, head, row tile) segment's chunks in a row, dealt to the
-// CTAs in equal contiguous parts: ragged lengths load all CTAs alike.  CTA c starts at
-// chunk floor(c * total / ctas).
+// The work is a row of segments (sequence, row tile, head), dealt to the CTAs in equal
+// contiguous parts so that ragged lengths load all CTAs alike.  A segment costs its
+// chunks and kOpen more for reading its queries, filling the ring and joining the warps
+// (measured with lengths up to 8192 of 64 sequences: without it the CTAs that got the
+// short ones took 1.25 times the mean).  CTA c starts at cost floor(c * total / ctas).
+constexpr uint32_t kOpen = 2;
+__device__ __forceinline__ uint32_t seq_cost(const Job &j, uint32_t s) {
+    const uint32_t n = seq_chunks(j, s);
+    return n ? n + kOpen : 0;
+}
 __device__ __forceinline__ uint64_t cta_start(uint64_t c, uint64_t total, uint32_t ctas) { return c * total / ctas; }
-__device__ __forceinline__ uint32_t cta_of(uint64_t chunk, uint64_t total, uint32_t ctas) {
-    return (uint32_t)(((chunk + 1) * ctas - 1) / total);
+__device__ __forceinline__ uint32_t cta_of(uint64_t at, uint64_t total, uint32_t ctas) {
+    return (uint32_t)(((at + 1) * ctas - 1) / total);
 }
 
-// Block-wide scan of the sequences' chunks: total, and the sequence that holds chunk
-// `x` (as a count of chunks times `per`) or, with find_seq, the first chunk of sequence x.
+// Block-wide scan of the sequences' costs (each `per` segments): the total, and the
+// sequence in which CTA x starts (by_cta) or the cost before sequence x.
 struct Located {
-    uint64_t total, first;  // chunks in all, first chunk of the located sequence
+    uint64_t total, first;  // cost in all, cost before the located sequence
     uint32_t seq;
 };
 template <uint32_t THREADS>
@@ -71,7 +78,7 @@ __device__ Located locate(const Job &j, uint32_t per, bool by_cta, uint64_t x, u
     const uint32_t each = (j.n_seq + THREADS - 1) / THREADS, s0 = min(threadIdx.x * each, j.n_seq),
                    s1 = min(s0 + each, j.n_seq);
     uint64_t mine = 0;
-    for (uint32_t s = s0; s < s1; ++s) mine += (uint64_t)seq_chunks(j, s) * per;
+    for (uint32_t s = s0; s < s1; ++s) mine += (uint64_t)seq_cost(j, s) * per;
     uint64_t scan = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -91,7 +98,7 @@ __device__ Located locate(const Job &j, uint32_t per, bool by_cta, uint64_t x, u
     if (threadIdx.x == 0) res = Located{total, 0, 0};
     __syncthreads();
     for (uint32_t s = s0; s < s1; ++s) {
-        const uint64_t n = (uint64_t)seq_chunks(j, s) * per;
+        const uint64_t n = (uint64_t)seq_cost(j, s) * per;
         if (by_cta ? (before <= at && at < before + n) : s == x) res.first = before, res.seq = s;
         before += n;
     }
@@ -135,9 +142,10 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
     return y;
 }
+// Of values with at most eight significant bits (codes): the upper halves of their f32.
 __device__ __forceinline__ uint32_t f16x2_to_bf16x2(uint32_t h) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-    return pack_bf16x2(f.x, f.y);
+    return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
 }
 // Four E8M0 bytes -> bf16x2 of bytes (0,1) and (2,3).
 __device__ __forceinline__ void e8m0x4_to_bf16(uint32_t w, uint32_t &lo, uint32_t &hi) {
@@ -471,19 +479,22 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
 
     const Located loc = locate<kWarps * 32>(job, per, true, blockIdx.x, scan, where);
     uint64_t at = cta_start(blockIdx.x, loc.total, job.ctas);
-    const uint64_t end = cta_start(blockIdx.x + 1, loc.total, job.ctas), begin = at;
+    const uint64_t end = cta_start(blockIdx.x + 1, loc.total, job.ctas);
     uint32_t seq = loc.seq;
     uint64_t seq_first = loc.first;
     while (at < end) {
-        uint32_t chunks = seq_chunks(job, seq);
-        while (chunks == 0 || at >= seq_first + (uint64_t)chunks * per) {
-            seq_first += (uint64_t)chunks * per;
-            chunks = seq_chunks(job, ++seq);
+        uint32_t cost = seq_cost(job, seq);
+        while (at >= seq_first + (uint64_t)cost * per) {
+            seq_first += (uint64_t)cost * per;
+            cost = seq_cost(job, ++seq);
         }
-        const uint32_t len = seq_len(job, seq);
+        const uint32_t len = seq_len(job, seq), chunks = cost - kOpen;
         const uint64_t in_seq = at - seq_first;
-        const uint32_t unit = (uint32_t)(in_seq / chunks), c0 = (uint32_t)(in_seq - (uint64_t)unit * chunks);
-        const uint32_t c1 = (uint32_t)min((uint64_t)chunks, (uint64_t)c0 + (end - at));
+        const uint32_t unit = (uint32_t)(in_seq / cost), x0 = (uint32_t)(in_seq - (uint64_t)unit * cost);
+        const uint32_t x1 = (uint32_t)min((uint64_t)cost, (uint64_t)x0 + (end - at));
+        at += x1 - x0;
+        const uint32_t c0 = max(x0, kOpen) - kOpen, c1 = max(x1, kOpen) - kOpen;
+        if (c0 == c1) continue;
         const uint32_t head = unit % p.c.n_kv, r0 = unit / p.c.n_kv * ROWS;
         const uint32_t rows = min(ROWS, job.rows - r0);
         const int32_t *table = job.pages + (uint64_t)seq * job.table_stride;
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         const bool whole = c0 == 0 && c1 == chunks;
         float *slot = nullptr;
         if (!whole) {
-            slot = job.slots + (uint64_t)(2 * blockIdx.x + (at > begin)) * ROWS * (HD + 2);
+            slot = job.slots + (uint64_t)(2 * blockIdx.x + (c0 == 0)) * ROWS * (HD + 2);
             if (threadIdx.x < ROWS) slot[2 * threadIdx.x] = top[threadIdx.x], slot[2 * threadIdx.x + 1] = sum[threadIdx.x];
             slot += 2 * ROWS;
         } else if (job.row_slots && threadIdx.x < rows) {
@@ -646,7 +657,6 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
                 }
             }
         }
-        at += c1 - c0;
     }
 }
 
@@ -687,7 +697,7 @@ __global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant_
         const Located loc = locate<HD>(job, per, false, seq, scan, where);
         const uint32_t chunks = seq_chunks(job, seq);
         if (chunks == 0) continue;
-        const uint64_t first = loc.first + (uint64_t)(r / tile_rows * p.c.n_kv + kvh) * chunks;
+        const uint64_t first = loc.first + (uint64_t)(r / tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
         const uint32_t ca = cta_of(first, loc.total, job.ctas), cb = cta_of(first + chunks - 1, loc.total, job.ctas);
         if (ca == cb) {
             if (!job.row_slots) {
@@ -699,9 +709,8 @@ __global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant_
             continue;
         }
         for (uint32_t c = ca + warp; c <= cb; c += W) {
-            const uint64_t start = cta_start(c, loc.total, job.ctas);
-            if (cta_start(c + 1, loc.total, job.ctas) == start) continue;
-            const float *slot = job.slots + (uint64_t)(2 * c + (start < first)) * tile_rows * (HD + 2);
+            if (c != ca && cta_start(c, loc.total, job.ctas) == cta_start(c + 1, loc.total, job.ctas)) continue;
+            const float *slot = job.slots + (uint64_t)(2 * c + (c == ca)) * tile_rows * (HD + 2);
             take(slot + 2 * (r % tile_rows), slot + 2 * tile_rows + r % tile_rows * HD);
         }
     }
@@ -739,7 +748,7 @@ Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uin
     pl.nq = column_tiles(prefix_len ? all : rows);
     const uint32_t sms = (uint32_t)num_sms(), slots = sms * min_ctas(hd, pl.nq);
     const uint64_t tr = 8 * pl.nq;
-    auto chunks = [](uint32_t n) { return ((uint64_t)n + kChunk - 1) / kChunk; };
+    auto chunks = [](uint32_t n) { return ((uint64_t)n + kChunk - 1) / kChunk; };  // CTAs beyond the chunks would idle
     const uint64_t own = chunks(max_len) * batch * n_kv * ((rows + tr - 1) / tr);
     pl.own_ctas = (uint32_t)(own < slots ? own : slots);
     pl.own_slots = 2ull * pl.own_ctas * tr * (hd + 2);
