@@ -17,6 +17,7 @@
 // products with the scales, and probabilities far below the maximum, need the range (a
 // dimension in which the largest position's code is 0 is made of those alone).
 #include "mxkv.cuh"
+#include "tc05.cuh"
 
 namespace fp4x {
 namespace mxkv {
@@ -30,6 +31,7 @@ constexpr float kLag = 8.0f;                   // how far (in powers of two) a s
 // pages (n_seq = batch), or all rows of the batch over the shared prefix (n_seq = 1).
 struct Job {
     uint32_t n_seq, rows, row_tiles, ctas;  // sequences, query rows per (sequence, KV head), tiles of them, grid
+    uint32_t tile_rows;                     // 8, 16 or 32: attn_mx_kernel; 128: attn_mx_tile_kernel
     const int32_t *pages, *lens;            // lens null: every sequence holds max_len positions
     uint32_t table_stride, max_len;
     float *slots;      // 2 per CTA: its part of a segment that began before it, and of one that it began
@@ -105,6 +107,40 @@ __device__ Located locate(const Job &j, uint32_t per, bool by_cta, uint64_t x, u
     __syncthreads();
     return res;
 }
+
+// The segments of one CTA in turn.
+struct Segment {
+    uint32_t seq, head, r0, rows;  // first query row of the tile and how many it has
+    uint32_t c0, c1, chunks, len;  // this CTA's chunks of the sequence's
+    __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == chunks; }
+};
+struct Segments {
+    uint64_t at, end, seq_first;
+    uint32_t seq, per;
+    __device__ __forceinline__ Segments(const Job &j, uint32_t n_kv, const Located &loc) {
+        at = cta_start(blockIdx.x, loc.total, j.ctas), end = cta_start(blockIdx.x + 1, loc.total, j.ctas);
+        seq_first = loc.first, seq = loc.seq, per = n_kv * j.row_tiles;
+    }
+    __device__ __forceinline__ bool next(const Job &j, uint32_t n_kv, Segment &s) {
+        while (at < end) {
+            uint32_t cost = seq_cost(j, seq);
+            while (at >= seq_first + (uint64_t)cost * per) {
+                seq_first += (uint64_t)cost * per;
+                cost = seq_cost(j, ++seq);
+            }
+            const uint64_t in_seq = at - seq_first;
+            const uint32_t unit = (uint32_t)(in_seq / cost), x0 = (uint32_t)(in_seq - (uint64_t)unit * cost);
+            const uint32_t x1 = (uint32_t)min((uint64_t)cost, (uint64_t)x0 + (end - at));
+            at += x1 - x0;
+            s.c0 = max(x0, kOpen) - kOpen, s.c1 = max(x1, kOpen) - kOpen;
+            if (s.c0 == s.c1) continue;
+            s.seq = seq, s.len = seq_len(j, seq), s.chunks = cost - kOpen;
+            s.head = unit % n_kv, s.r0 = unit / n_kv * j.tile_rows, s.rows = min(j.tile_rows, j.rows - s.r0);
+            return true;
+        }
+        return false;
+    }
+};
 
 // ---------------------------------------------------------------- fragments
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, uint32_t size, uint32_t bytes) {
@@ -478,25 +514,10 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
     const uint32_t per = p.c.n_kv * job.row_tiles;
 
     const Located loc = locate<kWarps * 32>(job, per, true, blockIdx.x, scan, where);
-    uint64_t at = cta_start(blockIdx.x, loc.total, job.ctas);
-    const uint64_t end = cta_start(blockIdx.x + 1, loc.total, job.ctas);
-    uint32_t seq = loc.seq;
-    uint64_t seq_first = loc.first;
-    while (at < end) {
-        uint32_t cost = seq_cost(job, seq);
-        while (at >= seq_first + (uint64_t)cost * per) {
-            seq_first += (uint64_t)cost * per;
-            cost = seq_cost(job, ++seq);
-        }
-        const uint32_t len = seq_len(job, seq), chunks = cost - kOpen;
-        const uint64_t in_seq = at - seq_first;
-        const uint32_t unit = (uint32_t)(in_seq / cost), x0 = (uint32_t)(in_seq - (uint64_t)unit * cost);
-        const uint32_t x1 = (uint32_t)min((uint64_t)cost, (uint64_t)x0 + (end - at));
-        at += x1 - x0;
-        const uint32_t c0 = max(x0, kOpen) - kOpen, c1 = max(x1, kOpen) - kOpen;
-        if (c0 == c1) continue;
-        const uint32_t head = unit % p.c.n_kv, r0 = unit / p.c.n_kv * ROWS;
-        const uint32_t rows = min(ROWS, job.rows - r0);
+    Segments segments(job, p.c.n_kv, loc);
+    Segment sg;
+    while (segments.next(job, p.c.n_kv, sg)) {
+        const uint32_t seq = sg.seq, len = sg.len, head = sg.head, r0 = sg.r0, rows = sg.rows, c0 = sg.c0, c1 = sg.c1;
         const int32_t *table = job.pages + (uint64_t)seq * job.table_stride;
 
         // this warp's tiles: c * kWarps + warp for c in [c0, c1), those that start below len
@@ -607,7 +628,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             top[threadIdx.x] = mx, sum[threadIdx.x] = l;
         }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == chunks;
+        const bool whole = sg.whole();
         float *slot = nullptr;
         if (!whole) {
             slot = job.slots + (uint64_t)(2 * blockIdx.x + (c0 == 0)) * ROWS * (HD + 2);
@@ -660,11 +681,440 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
     }
 }
 
+// ---------------------------------------------------------------- many rows: tcgen05
+// attn_mx_tile_kernel: 128 query rows of a KV head against tiles of TN positions on
+// tcgen05.  The codes are dequantised once per tile for all 128 rows:
+//   warps 4-11  codes -> bf16 (exact: at most four significant bits times a power of
+//               two) in shared memory, rows of 128 bytes with the 128-byte swizzle; the
+//               same image serves K (K-major) and V (MN-major);
+//   warp 12     S = Q K^T and O += P V, S of the next tile ahead of P V;
+//   warps 0-3   one thread per row: maximum, exp2, row sum; P as two bf16 terms (16
+//               bits; f32 queries: Q and P as three, 24 bits) back into tensor memory,
+//               from where it is the A operand.  O is rescaled only when a row's maximum
+//               grows by more than kLag powers of two.
+template <uint32_t HD, bool F32>
+struct Big {
+    static constexpr uint32_t TN = F32 ? 64 : 128, QT = F32 ? 3 : 1, PT = F32 ? 3 : 2;
+    static constexpr uint32_t REG = HD / 64;  // 64-dimension regions of an operand
+    static constexpr uint32_t Q_BYTES = QT * REG * 128 * 128, KV_BYTES = REG * TN * 128;
+    static constexpr uint32_t SMEM = Q_BYTES + 4 * KV_BYTES + 1024;
+    static constexpr uint32_t THREADS = 13 * 32, DEQ = 256;
+    // tensor memory columns: two S buffers (with their P), then O
+    static constexpr uint32_t S_COLS = F32 ? 160 : 128, O_COL = 2 * S_COLS, COLS = 512;
+    // first column of term z of P for positions 16 ks .. 16 ks + 15 (8 columns), from the buffer's start
+    static __device__ __forceinline__ uint32_t p_col(uint32_t z, uint32_t ks) {
+        return F32 ? 64 + 32 * z + 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks & 1);
+    }
+};
+
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// kind::f16 instruction descriptor: bf16 x bf16 -> f32, M = 128; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc_bf16(uint32_t n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+#define FP4X_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define FP4X_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+        : FP4X_R8(v, 0), FP4X_R8(v, 8), FP4X_R8(v, 16), FP4X_R8(v, 24)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        FP4X_I8(v, 0), FP4X_I8(v, 8), FP4X_I8(v, 16), FP4X_I8(v, 24)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        FP4X_I8(v, 0), FP4X_I8(v, 8)
+        : "memory");
+}
+#undef FP4X_R8
+#undef FP4X_I8
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Codes of one thread's task: chunks 2 pair and 2 pair + 1 of a position, and its scales.
+template <uint32_t FMT, uint32_t HD>
+struct Codes {
+    static constexpr uint32_t W = Row<FMT, HD>::CHUNK / 2, NB = HD / 32;
+    uint32_t w[W], scales;
+    __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *sc) {
+        load_words<W>(codes, w);
+        scales = NB == 4 ? __ldg(reinterpret_cast<const uint32_t *>(sc)) : __ldg(reinterpret_cast<const uint16_t *>(sc));
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (uint32_t i = 0; i < W; ++i) w[i] = 0;
+        scales = 0;
+    }
+    // -> the position's row in an operand image at `base` (region stride TN * 128 bytes)
+    template <uint32_t TN>
+    __device__ __forceinline__ void store(uint8_t *base, uint32_t pos, uint32_t pair) const {
+        uint32_t sc[NB / 2];
+#pragma unroll
+        for (uint32_t i = 0; i < NB / 2; ++i)
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, l;\n\t}"
+                : "=r"(sc[i])
+                : "r"(i ? scales >> 16 : scales));
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            const uint32_t s2 = __byte_perm(sc[b / 2], 0, b & 1 ? 0x3232 : 0x1010);
+            uint32_t f[4], y[4];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                if constexpr (FMT == FMT_FP8) {
+                    e4m3x4_to_f16(w[h * NB + b], f[2 * h], f[2 * h + 1]);
+                } else {
+                    uint32_t d[4];
+                    decode_word_f16(w[(h * NB + b) / 2], d);
+                    f[2 * h] = d[2 * (b & 1)], f[2 * h + 1] = d[2 * (b & 1) + 1];
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) y[i] = bmul2(f16x2_to_bf16x2(f[i]), s2);
+            const uint32_t c = ((b & 1) * 4 + pair) ^ (pos & 7);
+            *reinterpret_cast<uint4 *>(base + (b / 2) * TN * 128 + pos * 128 + c * 16) =
+                make_uint4(y[0], y[1], y[2], y[3]);
+        }
+    }
+};
+
+// A bounded wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
+    return __all_sync(~0u, mbar_wait_bounded(bar, phase));
+}
+
+template <uint32_t FMT, uint32_t HD, typename T>
+__global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
+    attn_mx_tile_kernel(const __grid_constant__ AttnParams p, bool prefix) {
+    constexpr bool F32 = sizeof(T) == 4;
+    using BG = Big<HD, F32>;
+    constexpr uint32_t TN = BG::TN, ROWS = 128, GROUPS = TN / 16;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t scan[BG::THREADS / 32 + 1];
+    __shared__ Located where;
+    __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], pvdone[2], done;
+    // bit i: positions 16 i .. of the tile lie in no page.  Four deep: tile t + 4 is written after S of tile t + 2,
+    // which waits for P V of tile t and so for the softmax warps that read tile t's word.
+    __shared__ uint32_t tmem_base, bad_groups[4];
+    uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
+    uint8_t *qs = smem, *ks = smem + BG::Q_BYTES, *vs = ks + 2 * BG::KV_BYTES;
+    const Job &job = prefix ? p.prefix : p.own;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(&kfull[i], BG::DEQ / 32), mbar_init(&vfull[i], BG::DEQ / 32);
+            mbar_init(&kempty[i], 1), mbar_init(&vempty[i], 1), mbar_init(&sfull[i], 1), mbar_init(&pvdone[i], 1);
+            mbar_init(&pready[i], 4);
+        }
+        mbar_init(&done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tc::tmem_alloc(&tmem_base, BG::COLS);
+        tc::tmem_relinquish();
+    }
+    const Located loc = locate<BG::THREADS>(job, p.c.n_kv * job.row_tiles, true, blockIdx.x, scan, where);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_base;
+    Segments segments(job, p.c.n_kv, loc);
+    Segment sg;
+    bool ok = true;    // a bounded wait ran out: leave (the others' waits run out too)
+    uint32_t tile = 0;  // tiles taken so far, over all segments
+
+    if (warp < 4) {
+        // ================================================= softmax: thread = row
+        const uint32_t row = threadIdx.x, lanes = (warp * 32) << 16;
+        while (ok && segments.next(job, p.c.n_kv, sg)) {
+            const RowAt ra = row_at(p, prefix, sg.seq, sg.head, sg.r0 + min(row, sg.rows - 1));
+            const int32_t limit =
+                prefix ? (int32_t)sg.len : (int32_t)sg.len - (int32_t)p.q_len + 1 + (int32_t)ra.step;
+            const int32_t low = __reduce_min_sync(~0u, limit);
+            const uint32_t stop = min(sg.c1 * kChunk, sg.len);
+            float m = kNoMax, l = 0.0f;
+            bool first_tile = true;
+            for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile) {
+                const uint32_t buf = tile & 1, ph = (tile >> 1) & 1, sb = tmem + lanes + buf * BG::S_COLS;
+                if (!(ok = warp_wait(&sfull[buf], ph))) break;
+                tc::fence_after_sync();
+                const uint32_t bad = *(volatile uint32_t *)&bad_groups[tile & 3];
+                const bool masked = (int32_t)(pos + TN) > low || bad;
+                const int32_t left = limit - (int32_t)pos;
+                auto mask = [&](uint32_t(&x)[32], uint32_t c) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i)
+                        if ((int32_t)(c * 32 + i) >= left || (bad >> (c * 2 + i / 16)) & 1)
+                            x[i] = __float_as_uint(-INFINITY);
+                };
+                float mx = -INFINITY;
+#pragma unroll
+                for (uint32_t c = 0; c < TN / 32; ++c) {
+                    uint32_t x[32];
+                    tmem_ld32(sb + c * 32, x);
+                    if (masked) mask(x, c);
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 2)
+                        mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                }
+                mx *= p.scale;
+                const bool grow = mx > m + kLag;
+                if (__any_sync(~0u, grow)) {
+                    const float mn = grow ? mx : m, f = ex2(m - mn);
+                    m = mn, l *= f;
+                    if (!first_tile) {
+                        const uint32_t pt = tile - 1;
+                        if (!(ok = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1))) break;
+                        tc::fence_after_sync();
+#pragma unroll
+                        for (uint32_t c = 0; c < HD / 32; ++c) {
+                            uint32_t x[32];
+                            tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                            tmem_st32(tmem + lanes + BG::O_COL + c * 32, x);
+                        }
+                    }
+                }
+                first_tile = false;
+#pragma unroll
+                for (uint32_t c = 0; c < TN / 32; ++c) {
+                    uint32_t x[32], y[16];
+                    tmem_ld32(sb + c * 32, x);
+                    if (masked) mask(x, c);
+                    float part = 0.0f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i) {
+                        const float e = ex2(fmaf(__uint_as_float(x[i]), p.scale, -m));
+                        part += e;
+                        x[i] = __float_as_uint(e);
+                    }
+                    l += part;
+#pragma unroll
+                    for (uint32_t z = 0; z < BG::PT; ++z) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            const float a = __uint_as_float(x[2 * i]), b = __uint_as_float(x[2 * i + 1]);
+                            y[i] = pack_bf16x2(a, b);
+                            x[2 * i] = __float_as_uint(a - __uint_as_float(y[i] << 16));
+                            x[2 * i + 1] = __float_as_uint(b - __uint_as_float(y[i] & 0xFFFF0000u));
+                        }
+                        tmem_st16(sb + BG::p_col(z, 2 * c), y);
+                    }
+                }
+                tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pready[buf]);
+            }
+            if (!ok) break;
+            const uint32_t pt = tile - 1;
+            if (!(ok = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1))) break;
+            tc::fence_after_sync();
+            const uint64_t out_row = (uint64_t)ra.token * p.n_heads + ra.head;
+            const bool whole = sg.whole(), live = row < sg.rows;
+            float *dst = nullptr;
+            if (!whole) {
+                dst = job.slots + (uint64_t)(2 * blockIdx.x + (sg.c0 == 0)) * ROWS * (HD + 2);
+                if (live) dst[2 * row] = m, dst[2 * row + 1] = l;
+                dst += 2 * ROWS + row * HD;
+            } else if (job.row_slots) {
+                dst = job.row_slots + out_row * (HD + 2);
+                if (live) dst[HD] = m, dst[HD + 1] = l;
+            }
+            const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+            for (uint32_t c = 0; c < HD / 32; ++c) {
+                uint32_t x[32];
+                tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
+                if (live) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 2) {
+                        const float a = __uint_as_float(x[i]), b = __uint_as_float(x[i + 1]);
+                        if (dst)
+                            store2<float>(dst + c * 32 + i, a, b);
+                        else
+                            store2<T>((T *)p.out + out_row * HD + c * 32 + i, a * inv, b * inv);
+                    }
+                }
+            }
+            tc::fence_before_sync();
+        }
+    } else if (warp < 12) {
+        // ================================================= codes -> bf16 images
+        const uint32_t id = threadIdx.x - 128, pair = id & 3;
+        // eight lanes of a store phase hold positions x and x + 4: all 32 banks
+        const uint32_t sub = (lane >> 2) & 7, pos0 = (id / 32) * 8 + (sub >> 1) + (sub & 1) * 4;
+        constexpr uint32_t TASKS = TN / 64;
+        const uint32_t off = pair * Codes<FMT, HD>::W * 4;
+        while (ok && segments.next(job, p.c.n_kv, sg)) {
+            const int32_t *table = job.pages + (uint64_t)sg.seq * job.table_stride;
+            const uint32_t start = sg.c0 * kChunk, stop = min(sg.c1 * kChunk, sg.len);
+            Codes<FMT, HD> kc[TASKS], vc[TASKS];
+            int32_t ids[TASKS];  // pages of the positions to load next
+            auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : 0; };
+            auto fetch = [&](Codes<FMT, HD> &cd, const uint8_t *codes, const uint8_t *scales, uint32_t pos, int32_t page) {
+                if (pos < stop && (uint32_t)page < p.c.n_pages) {
+                    const uint32_t r = pos & ((1u << p.c.page_shift) - 1);
+                    cd.load(codes + code_off<FMT, HD>(p.c, page, sg.head, r) + off,
+                            scales + scale_off<HD>(p.c, page, sg.head, r));
+                } else {
+                    cd.clear();
+                }
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < TASKS; ++i) ids[i] = page_of(start + pos0 + 64 * i);
+#pragma unroll
+            for (uint32_t i = 0; i < TASKS; ++i) {
+                fetch(kc[i], p.c.k, p.c.ks, start + pos0 + 64 * i, ids[i]);
+                fetch(vc[i], p.c.v, p.c.vs, start + pos0 + 64 * i, ids[i]);
+            }
+            // ---- query rows: after the previous segment's last S
+            if (tile && !(ok = warp_wait(&kempty[(tile - 1) & 1], ((tile - 1) >> 1) & 1))) break;
+            for (uint32_t i = id; i < ROWS * (HD / 8); i += BG::DEQ) {
+                const uint32_t r = i / (HD / 8), c = i % (HD / 8);
+                float x[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) x[j] = 0.0f;
+                if (r < sg.rows) {
+                    const RowAt ra = row_at(p, prefix, sg.seq, sg.head, sg.r0 + r);
+                    load8<T>((const T *)p.q + (uint64_t)ra.token * p.q_stride + ra.head * HD + c * 8, x);
+                }
+#pragma unroll
+                for (uint32_t z = 0; z < BG::QT; ++z) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        y[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+                        x[2 * j] -= __uint_as_float(y[j] << 16), x[2 * j + 1] -= __uint_as_float(y[j] & 0xFFFF0000u);
+                    }
+                    *reinterpret_cast<uint4 *>(qs + (z * BG::REG + c / 8) * 128 * 128 + r * 128 +
+                                               ((c & 7) ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            for (uint32_t pos = start; pos < stop; pos += TN, ++tile) {
+                const uint32_t st = tile & 1, use = tile >> 1;
+                int32_t next[TASKS];
+#pragma unroll
+                for (uint32_t i = 0; i < TASKS; ++i) next[i] = page_of(pos + TN + pos0 + 64 * i);
+                if (use && !(ok = warp_wait(&kempty[st], (use - 1) & 1))) break;
+#pragma unroll
+                for (uint32_t i = 0; i < TASKS; ++i) {
+                    kc[i].template store<TN>(ks + st * BG::KV_BYTES, pos0 + 64 * i, pair);
+                    fetch(kc[i], p.c.k, p.c.ks, pos + TN + pos0 + 64 * i, next[i]);
+                }
+                if (id < 32) {  // pages outside the cache: groups of 16 positions
+                    const uint32_t at = pos + 16 * lane;
+                    const bool out = lane < GROUPS && at < stop &&
+                                     (uint32_t)table[at >> p.c.page_shift] >= p.c.n_pages;
+                    const uint32_t bits = __ballot_sync(~0u, out);
+                    if (lane == 0) {
+                        bad_groups[tile & 3] = bits;
+                        if (bits) raise_device_error(DEVERR_BAD_ARG);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kfull[st]);
+                if (use && !(ok = warp_wait(&vempty[st], (use - 1) & 1))) break;
+#pragma unroll
+                for (uint32_t i = 0; i < TASKS; ++i) {
+                    vc[i].template store<TN>(vs + st * BG::KV_BYTES, pos0 + 64 * i, pair);
+                    fetch(vc[i], p.c.v, p.c.vs, pos + TN + pos0 + 64 * i, next[i]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vfull[st]);
+            }
+        }
+    } else if (lane == 0) {
+        // ================================================= one thread issues the MMAs
+        const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
+        constexpr uint32_t ID_S = idesc_bf16(TN, false), ID_O = idesc_bf16(HD, true);
+        uint32_t pv = 0;        // tiles whose P V has been issued
+        bool pv_first = true;   // the pending one opens its segment
+        auto issue_pv = [&]() {
+            const uint32_t st = pv & 1, ph = (pv >> 1) & 1;
+            if (!mbar_wait_bounded(&vfull[st], ph) || !mbar_wait_bounded(&pready[st], ph)) return false;
+            tc::fence_after_sync();
+            const uint32_t sb = tmem + st * BG::S_COLS, vb = va + st * BG::KV_BYTES;
+#pragma unroll 1
+            for (uint32_t k = 0; k < TN / 16; ++k) {
+                const uint64_t bd = tc::smem_desc(vb + k * 2048, TN * 128, 1024, tc::kLayoutSw128);
+#pragma unroll
+                for (uint32_t z = 0; z < BG::PT; ++z)
+                    mma_bf16_ts(tmem + BG::O_COL, sb + BG::p_col(z, k), bd, ID_O, !(pv_first && k == 0 && z == 0));
+            }
+            tc::commit(&vempty[st]);
+            tc::commit(&pvdone[st]);
+            ++pv;
+            return true;
+        };
+        bool pending = false, pending_first = false;
+        while (ok && segments.next(job, p.c.n_kv, sg)) {
+            const uint32_t start = sg.c0 * kChunk, stop = min(sg.c1 * kChunk, sg.len);
+            for (uint32_t pos = start; pos < stop; pos += TN, ++tile) {
+                const uint32_t st = tile & 1, ph = (tile >> 1) & 1;
+                // the S buffer holds the P of two tiles ago until its P V is done
+                if (tile >= 2 && !(ok = mbar_wait_bounded(&pvdone[st], ((tile >> 1) - 1) & 1))) break;
+                if (!(ok = mbar_wait_bounded(&kfull[st], ph))) break;
+                tc::fence_after_sync();
+                const uint32_t kb = ka + st * BG::KV_BYTES;
+#pragma unroll 1
+                for (uint32_t z = 0; z < BG::QT; ++z)
+#pragma unroll 1
+                    for (uint32_t k = 0; k < HD / 16; ++k)
+                        mma_bf16_ss(tmem + st * BG::S_COLS,
+                                    tc::desc_sw128(qa + (z * BG::REG + k / 4) * 128 * 128 + (k & 3) * 32),
+                                    tc::desc_sw128(kb + (k / 4) * TN * 128 + (k & 3) * 32), ID_S, z || k);
+                tc::commit(&kempty[st]);
+                tc::commit(&sfull[st]);
+                if (pending) {
+                    pv_first = pending_first;
+                    if (!(ok = issue_pv())) break;
+                }
+                pending = true, pending_first = pos == start;
+            }
+        }
+        if (ok && pending) {
+            pv_first = pending_first;
+            ok = issue_pv();
+        }
+        // everything issued has finished before tensor memory is given back
+        tc::commit(&done);
+        mbar_wait_bounded(&done, 0);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    if (warp == 12) tc::tmem_dealloc(tmem, BG::COLS);
+}
+
 // Joins the partial results of one output row: those of the CTAs that shared its
 // segment, and with a prefix those of both jobs.  A CTA of HD threads per row, each
 // warp takes every fourth (second) partial.
 template <uint32_t HD, typename T>
-__global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant__ AttnParams p, uint32_t tile_rows) {
+__global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr uint32_t W = HD / 32;
     __shared__ uint64_t scan[W + 1];
     __shared__ Located where;
@@ -693,7 +1143,7 @@ __global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant_
             direct = false;
             continue;
         }
-        const uint32_t per = p.c.n_kv * job.row_tiles;
+        const uint32_t per = p.c.n_kv * job.row_tiles, tile_rows = job.tile_rows;
         const Located loc = locate<HD>(job, per, false, seq, scan, where);
         const uint32_t chunks = seq_chunks(job, seq);
         if (chunks == 0) continue;
@@ -731,63 +1181,81 @@ __global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- host
-// Columns of a row tile: 8 per mma; up to 32 rows share one read of the codes.
-inline uint32_t column_tiles(uint64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// Rows of a tile: 8 per mma column tile; up to 32 rows share one read of the codes in
+// attn_mx_kernel, 128 in attn_mx_tile_kernel.
+inline uint32_t tile_rows_of(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
 
 struct Plan {
-    uint32_t nq;                   // column tiles of both jobs
+    uint32_t own_rows, prefix_rows;  // per tile
     uint32_t own_ctas, prefix_ctas;
     uint64_t own_slots, prefix_slots, row_slots;  // floats
 };
-inline uint32_t min_ctas(uint32_t hd, uint32_t nq) { return nq * hd <= 128 ? 2 : 1; }
+// CTAs of a job that run at once per SM: see Tile::MIN_CTAS.
+inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows) { return tile_rows * hd <= 1024 ? 2 : 1; }
 
 Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uint32_t q_len, uint32_t prefix_len,
                uint32_t max_len) {
     Plan pl = {};
-    const uint64_t group = n_heads / n_kv, rows = group * q_len, all = rows * batch;
-    pl.nq = column_tiles(prefix_len ? all : rows);
-    const uint32_t sms = (uint32_t)num_sms(), slots = sms * min_ctas(hd, pl.nq);
-    const uint64_t tr = 8 * pl.nq;
-    auto chunks = [](uint32_t n) { return ((uint64_t)n + kChunk - 1) / kChunk; };  // CTAs beyond the chunks would idle
-    const uint64_t own = chunks(max_len) * batch * n_kv * ((rows + tr - 1) / tr);
-    pl.own_ctas = (uint32_t)(own < slots ? own : slots);
-    pl.own_slots = 2ull * pl.own_ctas * tr * (hd + 2);
+    const uint64_t rows = (uint64_t)(n_heads / n_kv) * q_len, all = rows * batch;
+    const uint32_t sms = (uint32_t)num_sms();
+    auto job = [&](uint32_t seqs, uint32_t len, uint64_t r, uint32_t &tile_rows, uint32_t &ctas, uint64_t &slots) {
+        tile_rows = tile_rows_of(r);
+        const uint64_t chunks = ((uint64_t)len + kChunk - 1) / kChunk * seqs * n_kv * ((r + tile_rows - 1) / tile_rows);
+        const uint64_t room = (uint64_t)sms * ctas_per_sm(hd, tile_rows);
+        ctas = (uint32_t)(chunks < room ? chunks : room);  // more would idle
+        slots = 2ull * ctas * tile_rows * (hd + 2);
+    };
+    job(batch, max_len, rows, pl.own_rows, pl.own_ctas, pl.own_slots);
     if (prefix_len) {
-        const uint64_t pre = chunks(prefix_len) * n_kv * ((all + tr - 1) / tr);
-        pl.prefix_ctas = (uint32_t)(pre < slots ? pre : slots);
-        pl.prefix_slots = 2ull * pl.prefix_ctas * tr * (hd + 2);
+        job(1, prefix_len, all, pl.prefix_rows, pl.prefix_ctas, pl.prefix_slots);
         pl.row_slots = (uint64_t)batch * q_len * n_heads * (hd + 2);
     }
     return pl;
 }
 
-template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
-int launch_job(const char *who, cudaStream_t st, const AttnParams &p, bool prefix) {
-    using TT = Tile<FMT, HD, NQ, sizeof(T) == 4>;
-    auto kernel = attn_mx_kernel<FMT, HD, NQ, T>;
-    static bool ready[64] = {};
+template <typename K>
+int launch_with_smem(const char *who, cudaStream_t st, K kernel, bool (&ready)[64], uint32_t ctas, uint32_t threads,
+                     uint32_t smem, const AttnParams &p, bool prefix) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TT::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    kernel<<<(prefix ? p.prefix : p.own).ctas, kWarps * 32, TT::SMEM, st>>>(p, prefix);
+    kernel<<<ctas, threads, smem, st>>>(p, prefix);
     return check_launch(who);
 }
 
+template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
+int launch_stream(const char *who, cudaStream_t st, const AttnParams &p, bool prefix) {
+    using TT = Tile<FMT, HD, NQ, sizeof(T) == 4>;
+    static_assert(TT::MIN_CTAS == (8 * NQ * HD <= 1024 ? 2 : 1), "ctas_per_sm and the launch bounds agree");
+    static bool ready[64] = {};
+    return launch_with_smem(who, st, attn_mx_kernel<FMT, HD, NQ, T>, ready, (prefix ? p.prefix : p.own).ctas,
+                            kWarps * 32, TT::SMEM, p, prefix);
+}
 template <uint32_t FMT, uint32_t HD, typename T>
-int launch_all(const char *who, cudaStream_t st, const AttnParams &p, uint32_t nq, uint64_t rows) {
+int launch_tile(const char *who, cudaStream_t st, const AttnParams &p, bool prefix) {
+    using BG = Big<HD, sizeof(T) == 4>;
+    static bool ready[64] = {};
+    return launch_with_smem(who, st, attn_mx_tile_kernel<FMT, HD, T>, ready, (prefix ? p.prefix : p.own).ctas,
+                            BG::THREADS, BG::SMEM, p, prefix);
+}
+
+template <uint32_t FMT, uint32_t HD, typename T>
+int launch_all(const char *who, cudaStream_t st, const AttnParams &p, uint64_t rows) {
     int rc = FP4X_OK;
     for (int prefix = 1; prefix >= 0 && rc == FP4X_OK; --prefix) {
-        if (!(prefix ? p.prefix : p.own).ctas) continue;
-        rc = nq == 1   ? launch_job<FMT, HD, 1, T>(who, st, p, prefix)
-             : nq == 2 ? launch_job<FMT, HD, 2, T>(who, st, p, prefix)
-                       : launch_job<FMT, HD, 4, T>(who, st, p, prefix);
+        const Job &job = prefix ? p.prefix : p.own;
+        if (!job.ctas) continue;
+        rc = job.tile_rows == 8    ? launch_stream<FMT, HD, 1, T>(who, st, p, prefix)
+             : job.tile_rows == 16 ? launch_stream<FMT, HD, 2, T>(who, st, p, prefix)
+             : job.tile_rows == 32 ? launch_stream<FMT, HD, 4, T>(who, st, p, prefix)
+                                   : launch_tile<FMT, HD, T>(who, st, p, prefix);
     }
     if (rc != FP4X_OK) return rc;
-    const cudaError_t e = launch_pdl(attn_mx_join_kernel<HD, T>, dim3((uint32_t)rows), dim3(HD), 0, st, p, 8 * nq);
+    const cudaError_t e = launch_pdl(attn_mx_join_kernel<HD, T>, dim3((uint32_t)rows), dim3(HD), 0, st, p);
     if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
     return check_launch(who);
 }
@@ -824,18 +1292,21 @@ int launch_attn(const char *who, cudaStream_t st, const fp4x_mxkv *cache, uint32
     p.n_heads = n_heads, p.group = n_heads / p.c.n_kv, p.q_len = q_len;
     p.q = q, p.q_stride = q_stride, p.out = out;
     p.scale = 1.4426950408889634f / sqrtf((float)hd);
-    const uint32_t tr = 8 * pl.nq, own_rows = p.group * q_len, all = own_rows * batch;
-    p.own = Job{batch, own_rows, (own_rows + tr - 1) / tr, pl.own_ctas, page_table, lens, table_stride, max_len, ws,
-                prefix_len ? ws + pl.own_slots + pl.prefix_slots : nullptr};
-    p.prefix = Job{1, all, (all + tr - 1) / tr, pl.prefix_ctas, prefix_pages, nullptr, 0, prefix_len,
-                   ws + pl.own_slots, ws + pl.own_slots + pl.prefix_slots + pl.row_slots};
+    const uint32_t own_rows = p.group * q_len, all = own_rows * batch;
+    p.own = Job{batch, own_rows, (own_rows + pl.own_rows - 1) / pl.own_rows, pl.own_ctas, pl.own_rows, page_table, lens,
+                table_stride, max_len, ws, prefix_len ? ws + pl.own_slots + pl.prefix_slots : nullptr};
+    p.prefix = Job{};
+    if (prefix_len)
+        p.prefix = Job{1, all, (all + pl.prefix_rows - 1) / pl.prefix_rows, pl.prefix_ctas, pl.prefix_rows,
+                       prefix_pages, nullptr, 0, prefix_len, ws + pl.own_slots,
+                       ws + pl.own_slots + pl.prefix_slots + pl.row_slots};
     const bool f32 = dtype == FP4X_F32;
     if (cache->format == FP4X_MXFP8) {
-        if (hd == 64) return f32 ? launch_all<FMT_FP8, 64, float>(who, st, p, pl.nq, rows) : launch_all<FMT_FP8, 64, __nv_bfloat16>(who, st, p, pl.nq, rows);
-        return f32 ? launch_all<FMT_FP8, 128, float>(who, st, p, pl.nq, rows) : launch_all<FMT_FP8, 128, __nv_bfloat16>(who, st, p, pl.nq, rows);
+        if (hd == 64) return f32 ? launch_all<FMT_FP8, 64, float>(who, st, p, rows) : launch_all<FMT_FP8, 64, __nv_bfloat16>(who, st, p, rows);
+        return f32 ? launch_all<FMT_FP8, 128, float>(who, st, p, rows) : launch_all<FMT_FP8, 128, __nv_bfloat16>(who, st, p, rows);
     }
-    if (hd == 64) return f32 ? launch_all<FMT_FP4, 64, float>(who, st, p, pl.nq, rows) : launch_all<FMT_FP4, 64, __nv_bfloat16>(who, st, p, pl.nq, rows);
-    return f32 ? launch_all<FMT_FP4, 128, float>(who, st, p, pl.nq, rows) : launch_all<FMT_FP4, 128, __nv_bfloat16>(who, st, p, pl.nq, rows);
+    if (hd == 64) return f32 ? launch_all<FMT_FP4, 64, float>(who, st, p, rows) : launch_all<FMT_FP4, 64, __nv_bfloat16>(who, st, p, rows);
+    return f32 ? launch_all<FMT_FP4, 128, float>(who, st, p, rows) : launch_all<FMT_FP4, 128, __nv_bfloat16>(who, st, p, rows);
 }
 
 }  // namespace mxkv
