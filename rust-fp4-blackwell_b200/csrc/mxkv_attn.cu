@@ -36,6 +36,7 @@ struct Job {
     uint32_t table_stride, max_len;
     float *slots;      // 2 per CTA: its part of a segment that began before it, and of one that it began
     float *row_slots;  // one per output row for segments of one CTA (null: written to out)
+    uint64_t *starts;  // cost before every sequence, then the total: for the join (null: one sequence)
 };
 
 struct AttnParams {
@@ -63,20 +64,22 @@ __device__ __forceinline__ uint32_t seq_cost(const Job &j, uint32_t s) {
     const uint32_t n = seq_chunks(j, s);
     return n ? n + kOpen : 0;
 }
-__device__ __forceinline__ uint64_t cta_start(uint64_t c, uint64_t total, uint32_t ctas) { return c * total / ctas; }
+__device__ __forceinline__ uint64_t div(uint64_t a, uint64_t b) {  // a 64-bit division costs some hundred cycles
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+__device__ __forceinline__ uint64_t cta_start(uint64_t c, uint64_t total, uint32_t ctas) { return div(c * total, ctas); }
 __device__ __forceinline__ uint32_t cta_of(uint64_t at, uint64_t total, uint32_t ctas) {
-    return (uint32_t)(((at + 1) * ctas - 1) / total);
+    return (uint32_t)div((at + 1) * ctas - 1, total);
 }
 
 // Block-wide scan of the sequences' costs (each `per` segments): the total, and the
-// sequence in which CTA x starts (by_cta) or the cost before sequence x.
+// sequence in which this CTA starts.
 struct Located {
     uint64_t total, first;  // cost in all, cost before the located sequence
     uint32_t seq;
 };
 template <uint32_t THREADS>
-__device__ Located locate(const Job &j, uint32_t per, bool by_cta, uint64_t x, uint64_t (&buf)[THREADS / 32 + 1],
-                          Located &res) {
+__device__ Located locate(const Job &j, uint32_t per, uint64_t (&buf)[THREADS / 32 + 1], Located &res) {
     const uint32_t each = (j.n_seq + THREADS - 1) / THREADS, s0 = min(threadIdx.x * each, j.n_seq),
                    s1 = min(s0 + each, j.n_seq);
     uint64_t mine = 0;
@@ -96,12 +99,16 @@ __device__ Located locate(const Job &j, uint32_t per, bool by_cta, uint64_t x, u
         total += buf[w];
     }
     before += scan - mine;
-    const uint64_t at = by_cta ? cta_start(x, total, j.ctas) : 0;
-    if (threadIdx.x == 0) res = Located{total, 0, 0};
+    const uint64_t at = cta_start(blockIdx.x, total, j.ctas);
+    if (threadIdx.x == 0) {
+        res = Located{total, 0, 0};
+        if (j.starts && blockIdx.x == 0) j.starts[j.n_seq] = total;
+    }
     __syncthreads();
     for (uint32_t s = s0; s < s1; ++s) {
         const uint64_t n = (uint64_t)seq_cost(j, s) * per;
-        if (by_cta ? (before <= at && at < before + n) : s == x) res.first = before, res.seq = s;
+        if (before <= at && at < before + n) res.first = before, res.seq = s;
+        if (j.starts && blockIdx.x == 0) j.starts[s] = before;
         before += n;
     }
     __syncthreads();
@@ -129,7 +136,7 @@ struct Segments {
                 cost = seq_cost(j, ++seq);
             }
             const uint64_t in_seq = at - seq_first;
-            const uint32_t unit = (uint32_t)(in_seq / cost), x0 = (uint32_t)(in_seq - (uint64_t)unit * cost);
+            const uint32_t unit = (uint32_t)div(in_seq, cost), x0 = (uint32_t)(in_seq - (uint64_t)unit * cost);
             const uint32_t x1 = (uint32_t)min((uint64_t)cost, (uint64_t)x0 + (end - at));
             at += x1 - x0;
             s.c0 = max(x0, kOpen) - kOpen, s.c1 = max(x1, kOpen) - kOpen;
@@ -497,6 +504,7 @@ __device__ __forceinline__ void store2<__nv_bfloat16>(__nv_bfloat16 *p, float x,
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
 __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>::MIN_CTAS)
     attn_mx_kernel(const __grid_constant__ AttnParams p, bool prefix) {
+    pdl_launch_dependents();
     constexpr bool F32 = sizeof(T) == 4;
     using TT = Tile<FMT, HD, NQ, F32>;
     using R = Ring<FMT, HD>;
@@ -511,41 +519,41 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
     const uint32_t ring = smem_u32(smem) + warp * R::STAGES * R::STAGE;
     uint8_t *qbuf = smem + kWarps * R::STAGES * R::STAGE;
     float4 *merge = reinterpret_cast<float4 *>(qbuf + TT::Q_BYTES);
-    const uint32_t per = p.c.n_kv * job.row_tiles;
-
-    const Located loc = locate<kWarps * 32>(job, per, true, blockIdx.x, scan, where);
+    const Located loc = locate<kWarps * 32>(job, p.c.n_kv * job.row_tiles, scan, where);
     Segments segments(job, p.c.n_kv, loc);
-    Segment sg;
-    while (segments.next(job, p.c.n_kv, sg)) {
-        const uint32_t seq = sg.seq, len = sg.len, head = sg.head, r0 = sg.r0, rows = sg.rows, c0 = sg.c0, c1 = sg.c1;
-        const int32_t *table = job.pages + (uint64_t)seq * job.table_stride;
-
-        // this warp's tiles: c * kWarps + warp for c in [c0, c1), those that start below len
-        const uint32_t tiles = (len + 15) / 16;
-        uint32_t n_tiles = c1 - c0;
-        while (n_tiles && (c0 + n_tiles - 1) * kWarps + warp >= tiles) --n_tiles;
-        int32_t ids = 0;   // lane j: page of tile (j modulo 32)
-        uint32_t bad = 0;  // bit s: the page of the tile in stage s is outside the cache
-        auto load_ids = [&](uint32_t j0) {
-            const uint32_t j = j0 + lane;
-            ids = j < n_tiles ? table[((c0 + j) * kWarps + warp) * 16 >> p.c.page_shift] : 0;
-        };
-        auto issue = [&](uint32_t j) {
-            if ((j & 31) == 0 && j < n_tiles) load_ids(j);
-            if (j < n_tiles) {
-                const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
-                const int32_t page = __shfl_sync(~0u, ids, j & 31);
-                issue_tile<FMT, HD>(p.c, ring + j % R::STAGES * R::STAGE, page, head,
-                                    first & ((1u << p.c.page_shift) - 1), min(16u, len - first), lane);
-                const bool out = (uint32_t)page >= p.c.n_pages;
-                bad = (bad & ~(1u << j % R::STAGES)) | ((uint32_t)out << j % R::STAGES);
-                if (out && lane == 0) raise_device_error(DEVERR_BAD_ARG);
-            }
-            cp_async_commit();
-        };
-        __syncthreads();  // the previous segment's buffers are free
+    // The segment in work, as this warp sees it: its tiles are c * kWarps + warp for c in
+    // [c0, c1), those that start below len.
+    Segment sg = {};
+    uint32_t n_tiles = 0, bad = 0;  // bit s of bad: the page of the tile in stage s is outside the cache
+    int32_t ids = 0;                // lane j: page of tile (j modulo 32)
+    const int32_t *table = nullptr;
+    auto issue = [&](uint32_t j) {
+        if (j < n_tiles) {
+            if ((j & 31) == 0) ids = j + lane < n_tiles ? table[((sg.c0 + j + lane) * kWarps + warp) * 16 >> p.c.page_shift] : 0;
+            const uint32_t first = ((sg.c0 + j) * kWarps + warp) * 16;
+            const int32_t page = __shfl_sync(~0u, ids, j & 31);
+            issue_tile<FMT, HD>(p.c, ring + j % R::STAGES * R::STAGE, page, sg.head,
+                                first & ((1u << p.c.page_shift) - 1), min(16u, sg.len - first), lane);
+            const bool out = (uint32_t)page >= p.c.n_pages;
+            bad = (bad & ~(1u << j % R::STAGES)) | ((uint32_t)out << j % R::STAGES);
+            if (out && lane == 0) raise_device_error(DEVERR_BAD_ARG);
+        }
+        cp_async_commit();
+    };
+    auto open = [&]() {  // the next segment and its first copies
+        if (!segments.next(job, p.c.n_kv, sg)) return false;
+        table = job.pages + (uint64_t)sg.seq * job.table_stride;
+        const uint32_t tiles = (sg.len + 15) / 16;
+        n_tiles = sg.c1 - sg.c0;
+        while (n_tiles && (sg.c0 + n_tiles - 1) * kWarps + warp >= tiles) --n_tiles;
 #pragma unroll
         for (uint32_t j = 0; j < R::STAGES; ++j) issue(j);
+        return true;
+    };
+    bool more = open();
+    while (more) {
+        const Segment cur = sg;
+        const uint32_t seq = cur.seq, len = cur.len, head = cur.head, r0 = cur.r0, rows = cur.rows, c0 = cur.c0;
         // ---- query rows: scaled to a maximum in [2^14, 2^15), f16 (and the remainder's f16), fragment order
         for (uint32_t r = warp; r < ROWS; r += kWarps) {
             float x[HD / 32], amax = 0.0f;
@@ -607,6 +615,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             stage = stage + 1 == R::STAGES ? 0 : stage + 1;
             issue(j + R::STAGES);
         }
+        more = open();  // its first copies run under the joining of this one
         // ---- join the warps
 #pragma unroll
         for (uint32_t n = 0; n < NQ; ++n)
@@ -628,7 +637,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             top[threadIdx.x] = mx, sum[threadIdx.x] = l;
         }
         __syncthreads();
-        const bool whole = sg.whole();
+        const bool whole = cur.whole();
         float *slot = nullptr;
         if (!whole) {
             slot = job.slots + (uint64_t)(2 * blockIdx.x + (c0 == 0)) * ROWS * (HD + 2);
@@ -679,26 +688,29 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             }
         }
     }
+    // The own positions' kernel may start beside the prefix's; it ends after it, and the join waits for this one.
+    if (!prefix && p.prefix.ctas) pdl_wait();
 }
 
 // ---------------------------------------------------------------- many rows: tcgen05
 // attn_mx_tile_kernel: 128 query rows of a KV head against tiles of TN positions on
 // tcgen05.  The codes are dequantised once per tile for all 128 rows:
-//   warps 4-11  codes -> bf16 (exact: at most four significant bits times a power of
+//   warps 8-15  codes -> bf16 (exact: at most four significant bits times a power of
 //               two) in shared memory, rows of 128 bytes with the 128-byte swizzle; the
 //               same image serves K (K-major) and V (MN-major);
-//   warp 12     S = Q K^T and O += P V, S of the next tile ahead of P V;
-//   warps 0-3   one thread per row: maximum, exp2, row sum; P as two bf16 terms (16
-//               bits; f32 queries: Q and P as three, 24 bits) back into tensor memory,
-//               from where it is the A operand.  O is rescaled only when a row's maximum
-//               grows by more than kLag powers of two.
+//   warp 16     S = Q K^T and O += P V, S of the next tile ahead of P V;
+//   warps 0-7   two threads per row, half of the columns each: maximum (exchanged
+//               through shared memory), exp2, row sum; P as two bf16 terms (16 bits; f32
+//               queries: Q and P as three, 24 bits) back into tensor memory, from where
+//               it is the A operand.  O is rescaled only when a row's maximum grows by
+//               more than kLag powers of two.
 template <uint32_t HD, bool F32>
 struct Big {
     static constexpr uint32_t TN = F32 ? 64 : 128, QT = F32 ? 3 : 1, PT = F32 ? 3 : 2;
     static constexpr uint32_t REG = HD / 64;  // 64-dimension regions of an operand
     static constexpr uint32_t Q_BYTES = QT * REG * 128 * 128, KV_BYTES = REG * TN * 128;
     static constexpr uint32_t SMEM = Q_BYTES + 4 * KV_BYTES + 1024;
-    static constexpr uint32_t THREADS = 13 * 32, DEQ = 256;
+    static constexpr uint32_t THREADS = 17 * 32, DEQ = 256;
     // tensor memory columns: two S buffers (with their P), then O
     static constexpr uint32_t S_COLS = F32 ? 160 : 128, O_COL = 2 * S_COLS, COLS = 512;
     // first column of term z of P for positions 16 ks .. 16 ks + 15 (8 columns), from the buffer's start
@@ -798,6 +810,13 @@ struct Codes {
     }
 };
 
+// True in one lane of a converged warp (always the same one).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
 // A bounded wait of a whole warp, with one answer for all its lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
     return __all_sync(~0u, mbar_wait_bounded(bar, phase));
@@ -806,6 +825,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
 template <uint32_t FMT, uint32_t HD, typename T>
 __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     attn_mx_tile_kernel(const __grid_constant__ AttnParams p, bool prefix) {
+    pdl_launch_dependents();
     constexpr bool F32 = sizeof(T) == 4;
     using BG = Big<HD, F32>;
     constexpr uint32_t TN = BG::TN, ROWS = 128, GROUPS = TN / 16;
@@ -816,6 +836,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     // bit i: positions 16 i .. of the tile lie in no page.  Four deep: tile t + 4 is written after S of tile t + 2,
     // which waits for P V of tile t and so for the softmax warps that read tile t's word.
     __shared__ uint32_t tmem_base, bad_groups[4];
+    __shared__ float halfmax[2][2][ROWS], halfsum[2][ROWS];
     uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     uint8_t *qs = smem, *ks = smem + BG::Q_BYTES, *vs = ks + 2 * BG::KV_BYTES;
     const Job &job = prefix ? p.prefix : p.own;
@@ -824,28 +845,31 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&kfull[i], BG::DEQ / 32), mbar_init(&vfull[i], BG::DEQ / 32);
             mbar_init(&kempty[i], 1), mbar_init(&vempty[i], 1), mbar_init(&sfull[i], 1), mbar_init(&pvdone[i], 1);
-            mbar_init(&pready[i], 4);
+            mbar_init(&pready[i], 8);
         }
         mbar_init(&done, 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         tc::tmem_alloc(&tmem_base, BG::COLS);
         tc::tmem_relinquish();
     }
-    const Located loc = locate<BG::THREADS>(job, p.c.n_kv * job.row_tiles, true, blockIdx.x, scan, where);
+    const Located loc = locate<BG::THREADS>(job, p.c.n_kv * job.row_tiles, scan, where);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = tmem_base;
     Segments segments(job, p.c.n_kv, loc);
-    Segment sg;
+    Segment sg = {};
     bool ok = true;    // a bounded wait ran out: leave (the others' waits run out too)
     uint32_t tile = 0;  // tiles taken so far, over all segments
 
-    if (warp < 4) {
-        // ================================================= softmax: thread = row
-        const uint32_t row = threadIdx.x, lanes = (warp * 32) << 16;
+    if (warp < 8) {
+        // ================================================= softmax
+        const uint32_t quad = warp & 3, half = warp >> 2, row = quad * 32 + lane, lanes = (quad * 32) << 16;
+        constexpr uint32_t CH = TN / 64;  // 32-column pieces of a thread
+        // the two warps of 32 rows meet here; a failed wait is passed on as a NaN, so that both leave
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); };
         while (ok && segments.next(job, p.c.n_kv, sg)) {
             const RowAt ra = row_at(p, prefix, sg.seq, sg.head, sg.r0 + min(row, sg.rows - 1));
             const int32_t limit =
@@ -853,55 +877,64 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             const int32_t low = __reduce_min_sync(~0u, limit);
             const uint32_t stop = min(sg.c1 * kChunk, sg.len);
             float m = kNoMax, l = 0.0f;
-            bool first_tile = true;
+            bool first_tile = true, good = true;
             for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile) {
                 const uint32_t buf = tile & 1, ph = (tile >> 1) & 1, sb = tmem + lanes + buf * BG::S_COLS;
-                if (!(ok = warp_wait(&sfull[buf], ph))) break;
+                good = good && warp_wait(&sfull[buf], ph);
                 tc::fence_after_sync();
                 const uint32_t bad = *(volatile uint32_t *)&bad_groups[tile & 3];
                 const bool masked = (int32_t)(pos + TN) > low || bad;
                 const int32_t left = limit - (int32_t)pos;
-                auto mask = [&](uint32_t(&x)[32], uint32_t c) {
+                auto load = [&](uint32_t(&x)[32], uint32_t c) {
+                    tmem_ld32(sb + c * 32, x);
+                    if (masked) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i)
-                        if ((int32_t)(c * 32 + i) >= left || (bad >> (c * 2 + i / 16)) & 1)
-                            x[i] = __float_as_uint(-INFINITY);
+                        for (uint32_t i = 0; i < 32; ++i)
+                            if ((int32_t)(c * 32 + i) >= left || (bad >> (c * 2 + i / 16)) & 1)
+                                x[i] = __float_as_uint(-INFINITY);
+                    }
                 };
+                uint32_t x[32];  // the last piece stays for the exponentials
                 float mx = -INFINITY;
 #pragma unroll
-                for (uint32_t c = 0; c < TN / 32; ++c) {
-                    uint32_t x[32];
-                    tmem_ld32(sb + c * 32, x);
-                    if (masked) mask(x, c);
+                for (uint32_t c = 0; c < CH; ++c) {
+                    load(x, half * CH + c);
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 2)
                         mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
                 }
-                mx *= p.scale;
+                halfmax[tile & 1][half][row] = good ? mx : __uint_as_float(0x7FC00000u);
+                meet();
+                const float other = halfmax[tile & 1][half ^ 1][row];
+                if (__any_sync(~0u, !good || other != other)) {
+                    ok = false;
+                    break;
+                }
+                mx = fmaxf(mx, other) * p.scale;
                 const bool grow = mx > m + kLag;
                 if (__any_sync(~0u, grow)) {
                     const float mn = grow ? mx : m, f = ex2(m - mn);
                     m = mn, l *= f;
                     if (!first_tile) {
                         const uint32_t pt = tile - 1;
-                        if (!(ok = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1))) break;
+                        good = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
                         tc::fence_after_sync();
+#pragma unroll 1
+                        for (uint32_t c = 0; c < HD / 64; ++c) {
+                            const uint32_t at = tmem + lanes + BG::O_COL + (half * (HD / 64) + c) * 32;
+                            uint32_t y[32];
+                            tmem_ld32(at, y);
 #pragma unroll
-                        for (uint32_t c = 0; c < HD / 32; ++c) {
-                            uint32_t x[32];
-                            tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
-#pragma unroll
-                            for (uint32_t i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
-                            tmem_st32(tmem + lanes + BG::O_COL + c * 32, x);
+                            for (uint32_t i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                            tmem_st32(at, y);
                         }
                     }
                 }
                 first_tile = false;
 #pragma unroll
-                for (uint32_t c = 0; c < TN / 32; ++c) {
-                    uint32_t x[32], y[16];
-                    tmem_ld32(sb + c * 32, x);
-                    if (masked) mask(x, c);
+                for (uint32_t cc = 0; cc < CH; ++cc) {
+                    const uint32_t c = half * CH + (CH - 1 - cc);
+                    if (cc) load(x, c);
                     float part = 0.0f;
 #pragma unroll
                     for (uint32_t i = 0; i < 32; ++i) {
@@ -912,6 +945,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                     l += part;
 #pragma unroll
                     for (uint32_t z = 0; z < BG::PT; ++z) {
+                        uint32_t y[16];
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) {
                             const float a = __uint_as_float(x[2 * i]), b = __uint_as_float(x[2 * i + 1]);
@@ -929,22 +963,25 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             }
             if (!ok) break;
             const uint32_t pt = tile - 1;
-            if (!(ok = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1))) break;
+            good = good && warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
             tc::fence_after_sync();
+            halfsum[half][row] = l;
+            meet();
+            l = halfsum[0][row] + halfsum[1][row];
             const uint64_t out_row = (uint64_t)ra.token * p.n_heads + ra.head;
             const bool whole = sg.whole(), live = row < sg.rows;
             float *dst = nullptr;
             if (!whole) {
                 dst = job.slots + (uint64_t)(2 * blockIdx.x + (sg.c0 == 0)) * ROWS * (HD + 2);
-                if (live) dst[2 * row] = m, dst[2 * row + 1] = l;
+                if (live && !half) dst[2 * row] = m, dst[2 * row + 1] = l;
                 dst += 2 * ROWS + row * HD;
             } else if (job.row_slots) {
                 dst = job.row_slots + out_row * (HD + 2);
-                if (live) dst[HD] = m, dst[HD + 1] = l;
+                if (live && !half) dst[HD] = m, dst[HD + 1] = l;
             }
             const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-#pragma unroll
-            for (uint32_t c = 0; c < HD / 32; ++c) {
+#pragma unroll 1
+            for (uint32_t c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
                 if (live) {
@@ -959,10 +996,11 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
             }
             tc::fence_before_sync();
+            ok = good;
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ================================================= codes -> bf16 images
-        const uint32_t id = threadIdx.x - 128, pair = id & 3;
+        const uint32_t id = threadIdx.x - 256, pair = id & 3;
         // eight lanes of a store phase hold positions x and x + 4: all 32 banks
         const uint32_t sub = (lane >> 2) & 7, pos0 = (id / 32) * 8 + (sub >> 1) + (sub & 1) * 4;
         constexpr uint32_t TASKS = TN / 64;
@@ -1047,128 +1085,159 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 if (lane == 0) mbar_arrive(&vfull[st]);
             }
         }
-    } else if (lane == 0) {
-        // ================================================= one thread issues the MMAs
+    } else {
+        // ================================================= the MMAs
+        // The whole warp runs the loop and one elected lane issues: the operands then are
+        // warp-uniform values.  Issued from a branch on the lane number, an MMA took some
+        // 200 cycles instead of its 64.
         const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
         constexpr uint32_t ID_S = idesc_bf16(TN, false), ID_O = idesc_bf16(HD, true);
-        uint32_t pv = 0;        // tiles whose P V has been issued
-        bool pv_first = true;   // the pending one opens its segment
+        uint32_t pv = 0;  // tiles whose P V has been issued
+        bool pending = false, opens = false;  // a tile waits for its P V; it is its segment's first
         auto issue_pv = [&]() {
             const uint32_t st = pv & 1, ph = (pv >> 1) & 1;
-            if (!mbar_wait_bounded(&vfull[st], ph) || !mbar_wait_bounded(&pready[st], ph)) return false;
+            if (!warp_wait(&vfull[st], ph) || !warp_wait(&pready[st], ph)) return false;
             tc::fence_after_sync();
-            const uint32_t sb = tmem + st * BG::S_COLS, vb = va + st * BG::KV_BYTES;
-#pragma unroll 1
-            for (uint32_t k = 0; k < TN / 16; ++k) {
-                const uint64_t bd = tc::smem_desc(vb + k * 2048, TN * 128, 1024, tc::kLayoutSw128);
+            const uint32_t sb = tmem + st * BG::S_COLS;
+            const uint64_t bd = tc::smem_desc(va + st * BG::KV_BYTES, TN * 128, 1024, tc::kLayoutSw128);
+            if (elect_one()) {
 #pragma unroll
-                for (uint32_t z = 0; z < BG::PT; ++z)
-                    mma_bf16_ts(tmem + BG::O_COL, sb + BG::p_col(z, k), bd, ID_O, !(pv_first && k == 0 && z == 0));
+                for (uint32_t k = 0; k < TN / 16; ++k)
+#pragma unroll
+                    for (uint32_t z = 0; z < BG::PT; ++z)
+                        mma_bf16_ts(tmem + BG::O_COL, sb + BG::p_col(z, k), bd + k * (2048 >> 4), ID_O,
+                                    k || z ? 1u : !opens);
+                tc::commit(&vempty[st]);
+                tc::commit(&pvdone[st]);
             }
-            tc::commit(&vempty[st]);
-            tc::commit(&pvdone[st]);
+            __syncwarp();
             ++pv;
             return true;
         };
-        bool pending = false, pending_first = false;
         while (ok && segments.next(job, p.c.n_kv, sg)) {
             const uint32_t start = sg.c0 * kChunk, stop = min(sg.c1 * kChunk, sg.len);
             for (uint32_t pos = start; pos < stop; pos += TN, ++tile) {
                 const uint32_t st = tile & 1, ph = (tile >> 1) & 1;
                 // the S buffer holds the P of two tiles ago until its P V is done
-                if (tile >= 2 && !(ok = mbar_wait_bounded(&pvdone[st], ((tile >> 1) - 1) & 1))) break;
-                if (!(ok = mbar_wait_bounded(&kfull[st], ph))) break;
+                if (tile >= 2 && !(ok = warp_wait(&pvdone[st], ((tile >> 1) - 1) & 1))) break;
+                if (!(ok = warp_wait(&kfull[st], ph))) break;
                 tc::fence_after_sync();
-                const uint32_t kb = ka + st * BG::KV_BYTES;
-#pragma unroll 1
-                for (uint32_t z = 0; z < BG::QT; ++z)
-#pragma unroll 1
-                    for (uint32_t k = 0; k < HD / 16; ++k)
-                        mma_bf16_ss(tmem + st * BG::S_COLS,
-                                    tc::desc_sw128(qa + (z * BG::REG + k / 4) * 128 * 128 + (k & 3) * 32),
-                                    tc::desc_sw128(kb + (k / 4) * TN * 128 + (k & 3) * 32), ID_S, z || k);
-                tc::commit(&kempty[st]);
-                tc::commit(&sfull[st]);
-                if (pending) {
-                    pv_first = pending_first;
-                    if (!(ok = issue_pv())) break;
+                const uint64_t ad = tc::desc_sw128(qa), bd = tc::desc_sw128(ka + st * BG::KV_BYTES);
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t z = 0; z < BG::QT; ++z)
+#pragma unroll
+                        for (uint32_t k = 0; k < HD / 16; ++k)
+                            mma_bf16_ss(tmem + st * BG::S_COLS,
+                                        ad + (((z * BG::REG + k / 4) * 128 * 128 + (k & 3) * 32) >> 4),
+                                        bd + (((k / 4) * TN * 128 + (k & 3) * 32) >> 4), ID_S, z || k);
+                    tc::commit(&kempty[st]);
+                    tc::commit(&sfull[st]);
                 }
-                pending = true, pending_first = pos == start;
+                __syncwarp();
+                if (pending && !(ok = issue_pv())) break;
+                pending = true, opens = pos == start;
             }
         }
-        if (ok && pending) {
-            pv_first = pending_first;
-            ok = issue_pv();
-        }
+        if (ok && pending) ok = issue_pv();
         // everything issued has finished before tensor memory is given back
-        tc::commit(&done);
-        mbar_wait_bounded(&done, 0);
+        if (elect_one()) tc::commit(&done);
+        __syncwarp();
+        warp_wait(&done, 0);
     }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    if (warp == 12) tc::tmem_dealloc(tmem, BG::COLS);
+    if (warp == 16) tc::tmem_dealloc(tmem, BG::COLS);
+    if (!prefix && p.prefix.ctas) pdl_wait();
 }
 
 // Joins the partial results of one output row: those of the CTAs that shared its
-// segment, and with a prefix those of both jobs.  A CTA of HD threads per row, each
-// warp takes every fourth (second) partial.
+// segment, and with a prefix those of both jobs.  Four warps take the partials in turn,
+// four loads in flight each; a row that one CTA wrote whole has nothing to join.
 template <uint32_t HD, typename T>
-__global__ void __launch_bounds__(HD) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr uint32_t W = HD / 32;
-    __shared__ uint64_t scan[W + 1];
-    __shared__ Located where;
+__global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr uint32_t W = 4, V = HD / 32;  // a lane holds V dimensions
     __shared__ float sm[W], sl[W], so[W][HD];
-    pdl_wait();
     const uint32_t row = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t token = row / p.n_heads, head = row % p.n_heads, kvh = head / p.group;
-    float m = kNoMax, l = 0.0f, o[W];  // lane holds dimensions lane * W ..
+    pdl_wait();
+    // partials of each job: the row's slot, or its place in the slots of CTAs ca..cb
+    uint32_t n[2] = {0, 0}, ca[2] = {0, 0};
+    bool one[2] = {false, false};
+    uint64_t total[2] = {0, 0};
 #pragma unroll
-    for (uint32_t i = 0; i < W; ++i) o[i] = 0.0f;
-    auto take = [&](const float *ml, const float *po) {
-        const float pm = ml[0], pl = ml[1], mn = fmaxf(m, pm), f0 = exp2f(m - mn), f1 = exp2f(pm - mn);
-        l = l * f0 + pl * f1;
-#pragma unroll
-        for (uint32_t i = 0; i < W; ++i) o[i] = o[i] * f0 + po[lane * W + i] * f1;
-        m = mn;
-    };
-    bool direct = false;
-#pragma unroll 1
     for (uint32_t which = 0; which < 2; ++which) {
         const Job &job = which ? p.prefix : p.own;
-        if (which && !job.ctas) break;
+        if (!job.ctas) continue;
         const uint32_t seq = which ? 0 : token / p.q_len;
         const uint32_t r = which ? token * p.group + head % p.group : token % p.q_len * p.group + head % p.group;
-        if (job.ctas == 0) {  // no positions of their own in the whole batch
-            direct = false;
-            continue;
-        }
-        const uint32_t per = p.c.n_kv * job.row_tiles, tile_rows = job.tile_rows;
-        const Located loc = locate<HD>(job, per, false, seq, scan, where);
         const uint32_t chunks = seq_chunks(job, seq);
         if (chunks == 0) continue;
-        const uint64_t first = loc.first + (uint64_t)(r / tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
-        const uint32_t ca = cta_of(first, loc.total, job.ctas), cb = cta_of(first + chunks - 1, loc.total, job.ctas);
-        if (ca == cb) {
-            if (!job.row_slots) {
-                direct = true;
-            } else if (warp == 0) {
-                const float *rs = job.row_slots + (uint64_t)row * (HD + 2);
-                take(rs + HD, rs);
+        total[which] = which ? (uint64_t)seq_cost(job, 0) * p.c.n_kv * job.row_tiles : job.starts[job.n_seq];
+        const uint64_t first = (which ? 0 : job.starts[seq]) +
+                               (uint64_t)(r / job.tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
+        ca[which] = cta_of(first, total[which], job.ctas);
+        n[which] = cta_of(first + chunks - 1, total[which], job.ctas) - ca[which] + 1;
+        one[which] = n[which] == 1;
+        if (one[which] && !job.row_slots) return;  // written whole (without a prefix)
+    }
+    float m = kNoMax, l = 0.0f, o[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) o[i] = 0.0f;
+    constexpr uint32_t U = 4;
+    for (uint32_t k0 = warp; k0 < n[0] + n[1]; k0 += W * U) {
+        float pm[U], pl[U], po[U][V];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t k = k0 + u * W;
+            pm[u] = kNoMax, pl[u] = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) po[u][i] = 0.0f;
+            if (k >= n[0] + n[1]) continue;
+            const uint32_t which = k >= n[0], at = which ? k - n[0] : k;
+            const Job &job = which ? p.prefix : p.own;
+            const float *ml, *src;
+            if (one[which]) {
+                src = job.row_slots + (uint64_t)row * (HD + 2), ml = src + HD;
+            } else {
+                const uint32_t c = ca[which] + at, tr = job.tile_rows;
+                // a CTA without work of its own (more CTAs than cost)
+                if (total[which] < job.ctas && at &&
+                    cta_start(c, total[which], job.ctas) == cta_start(c + 1, total[which], job.ctas))
+                    continue;
+                const uint32_t r = which ? token * p.group + head % p.group : token % p.q_len * p.group + head % p.group;
+                const float *slot = job.slots + (uint64_t)(2 * c + (at == 0)) * tr * (HD + 2);
+                ml = slot + 2 * (r % tr), src = slot + 2 * tr + r % tr * HD;
             }
-            continue;
+            const float2 x = *reinterpret_cast<const float2 *>(ml);
+            pm[u] = x.x, pl[u] = x.y;
+#pragma unroll
+            for (uint32_t i = 0; i < V; i += 2) {
+                const float2 y = *reinterpret_cast<const float2 *>(src + lane * V + i);
+                po[u][i] = y.x, po[u][i + 1] = y.y;
+            }
         }
-        for (uint32_t c = ca + warp; c <= cb; c += W) {
-            if (c != ca && cta_start(c, loc.total, job.ctas) == cta_start(c + 1, loc.total, job.ctas)) continue;
-            const float *slot = job.slots + (uint64_t)(2 * c + (c == ca)) * tile_rows * (HD + 2);
-            take(slot + 2 * (r % tile_rows), slot + 2 * tile_rows + r % tile_rows * HD);
+        float mn = m;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+        const float f = exp2f(m - mn);
+        l *= f, m = mn;
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const float g = exp2f(pm[u] - mn);
+            l += pl[u] * g;
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) o[i] += po[u][i] * g;
         }
     }
-    if (direct) return;
     if (lane == 0) sm[warp] = m, sl[warp] = l;
 #pragma unroll
-    for (uint32_t i = 0; i < W; ++i) so[warp][lane * W + i] = o[i];
+    for (uint32_t i = 0; i < V; ++i) so[warp][lane * V + i] = o[i];
     __syncthreads();
+    if (threadIdx.x >= HD) return;
     float mx = kNoMax, sum = 0.0f, acc = 0.0f;
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) mx = fmaxf(mx, sm[w]);
@@ -1188,7 +1257,7 @@ inline uint32_t tile_rows_of(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 
 struct Plan {
     uint32_t own_rows, prefix_rows;  // per tile
     uint32_t own_ctas, prefix_ctas;
-    uint64_t own_slots, prefix_slots, row_slots;  // floats
+    uint64_t own_slots, prefix_slots, row_slots, starts;  // floats
 };
 // CTAs of a job that run at once per SM: see Tile::MIN_CTAS.
 inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows) { return tile_rows * hd <= 1024 ? 2 : 1; }
@@ -1206,6 +1275,7 @@ Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uin
         slots = 2ull * ctas * tile_rows * (hd + 2);
     };
     job(batch, max_len, rows, pl.own_rows, pl.own_ctas, pl.own_slots);
+    pl.starts = ((uint64_t)batch + 2) / 2 * 4;
     if (prefix_len) {
         job(1, prefix_len, all, pl.prefix_rows, pl.prefix_ctas, pl.prefix_slots);
         pl.row_slots = (uint64_t)batch * q_len * n_heads * (hd + 2);
@@ -1223,7 +1293,14 @@ int launch_with_smem(const char *who, cudaStream_t st, K kernel, bool (&ready)[6
         if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    kernel<<<ctas, threads, smem, st>>>(p, prefix);
+    // beside the prefix's kernel, which it does not read from
+    const bool beside = !prefix && p.prefix.ctas;
+    if (beside) {
+        const cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(threads), smem, st, p, prefix);
+        if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
+    } else {
+        kernel<<<ctas, threads, smem, st>>>(p, prefix);
+    }
     return check_launch(who);
 }
 
@@ -1255,7 +1332,7 @@ int launch_all(const char *who, cudaStream_t st, const AttnParams &p, uint64_t r
                                    : launch_tile<FMT, HD, T>(who, st, p, prefix);
     }
     if (rc != FP4X_OK) return rc;
-    const cudaError_t e = launch_pdl(attn_mx_join_kernel<HD, T>, dim3((uint32_t)rows), dim3(HD), 0, st, p);
+    const cudaError_t e = launch_pdl(attn_mx_join_kernel<HD, T>, dim3((uint32_t)rows), dim3(128), 0, st, p);
     if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
     return check_launch(who);
 }
@@ -1285,21 +1362,21 @@ int launch_attn(const char *who, cudaStream_t st, const fp4x_mxkv *cache, uint32
                  "%s: rows of q and out must be 16-byte aligned", who);
     FP4X_REQUIRE(q_stride >= (uint64_t)n_heads * hd, "%s: q_stride below n_heads * head_dim", who);
     const Plan pl = make_plan(p.c.n_kv, hd, batch, n_heads, q_len, prefix_len, max_len);
-    const size_t need = (pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float);
+    const size_t need = (pl.starts + pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float);
     FP4X_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
                  "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need, workspace_bytes);
-    float *ws = (float *)workspace;
+    float *ws = (float *)workspace + pl.starts;
     p.n_heads = n_heads, p.group = n_heads / p.c.n_kv, p.q_len = q_len;
     p.q = q, p.q_stride = q_stride, p.out = out;
     p.scale = 1.4426950408889634f / sqrtf((float)hd);
     const uint32_t own_rows = p.group * q_len, all = own_rows * batch;
     p.own = Job{batch, own_rows, (own_rows + pl.own_rows - 1) / pl.own_rows, pl.own_ctas, pl.own_rows, page_table, lens,
-                table_stride, max_len, ws, prefix_len ? ws + pl.own_slots + pl.prefix_slots : nullptr};
+                table_stride, max_len, ws, prefix_len ? ws + pl.own_slots + pl.prefix_slots : nullptr, (uint64_t *)workspace};
     p.prefix = Job{};
     if (prefix_len)
         p.prefix = Job{1, all, (all + pl.prefix_rows - 1) / pl.prefix_rows, pl.prefix_ctas, pl.prefix_rows,
                        prefix_pages, nullptr, 0, prefix_len, ws + pl.own_slots,
-                       ws + pl.own_slots + pl.prefix_slots + pl.row_slots};
+                       ws + pl.own_slots + pl.prefix_slots + pl.row_slots, nullptr};
     const bool f32 = dtype == FP4X_F32;
     if (cache->format == FP4X_MXFP8) {
         if (hd == 64) return f32 ? launch_all<FMT_FP8, 64, float>(who, st, p, rows) : launch_all<FMT_FP8, 64, __nv_bfloat16>(who, st, p, rows);
@@ -1319,7 +1396,7 @@ extern "C" size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t 
     if (!cache || !cache->n_kv_heads || n_heads < cache->n_kv_heads) return 0;
     const mxkv::Plan pl =
         mxkv::make_plan(cache->n_kv_heads, cache->head_dim, batch, n_heads, q_len, prefix_len, max_len);
-    return (size_t)((pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float));
+    return (size_t)((pl.starts + pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float));
 }
 
 extern "C" int llama_attn_paged_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
