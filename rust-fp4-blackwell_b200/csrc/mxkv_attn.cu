@@ -207,6 +207,23 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ float pow2(int e) {  // 2^e, -126 <= e <= 127
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
@@ -935,23 +952,30 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 for (uint32_t cc = 0; cc < CH; ++cc) {
                     const uint32_t c = half * CH + (CH - 1 - cc);
                     if (cc) load(x, c);
-                    float part = 0.0f;
+                    float2 part = {0.0f, 0.0f};
+                    const float2 sc2 = {p.scale, p.scale}, m2 = {-m, -m};
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i) {
-                        const float e = ex2(fmaf(__uint_as_float(x[i]), p.scale, -m));
-                        part += e;
-                        x[i] = __float_as_uint(e);
+                    for (uint32_t i = 0; i < 32; i += 2) {
+                        float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, m2);
+                        e = make_float2(ex2(e.x), ex2(e.y));
+                        part = add2(part, e);
+                        x[i] = __float_as_uint(e.x), x[i + 1] = __float_as_uint(e.y);
                     }
-                    l += part;
+                    l += part.x + part.y;
 #pragma unroll
                     for (uint32_t z = 0; z < BG::PT; ++z) {
                         uint32_t y[16];
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) {
-                            const float a = __uint_as_float(x[2 * i]), b = __uint_as_float(x[2 * i + 1]);
-                            y[i] = pack_bf16x2(a, b);
-                            x[2 * i] = __float_as_uint(a - __uint_as_float(y[i] << 16));
-                            x[2 * i + 1] = __float_as_uint(b - __uint_as_float(y[i] & 0xFFFF0000u));
+                            const float2 e = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                            if (z + 1 == BG::PT) {
+                                y[i] = pack_bf16x2(e.x, e.y);
+                            } else {  // the term cut off, not rounded: its upper half is the term
+                                y[i] = __byte_perm(x[2 * i], x[2 * i + 1], 0x7632);
+                                const float2 r = add2(e, make_float2(-__uint_as_float(x[2 * i] & 0xFFFF0000u),
+                                                                     -__uint_as_float(x[2 * i + 1] & 0xFFFF0000u)));
+                                x[2 * i] = __float_as_uint(r.x), x[2 * i + 1] = __float_as_uint(r.y);
+                            }
                         }
                         tmem_st16(sb + BG::p_col(z, 2 * c), y);
                     }
@@ -1009,23 +1033,29 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             const int32_t *table = job.pages + (uint64_t)sg.seq * job.table_stride;
             const uint32_t start = sg.c0 * kChunk, stop = min(sg.c1 * kChunk, sg.len);
             Codes<FMT, HD> kc[TASKS], vc[TASKS];
-            int32_t ids[TASKS];  // pages of the positions to load next
-            auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : 0; };
-            auto fetch = [&](Codes<FMT, HD> &cd, const uint8_t *codes, const uint8_t *scales, uint32_t pos, int32_t page) {
-                if (pos < stop && (uint32_t)page < p.c.n_pages) {
-                    const uint32_t r = pos & ((1u << p.c.page_shift) - 1);
-                    cd.load(codes + code_off<FMT, HD>(p.c, page, sg.head, r) + off,
-                            scales + scale_off<HD>(p.c, page, sg.head, r));
-                } else {
+            // where a position's row lies, in K and V alike; not in the cache or past the end: no row
+            struct Place {
+                uint64_t codes, scales;
+                bool row;
+            } at[TASKS];
+            auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : -1; };
+            auto place = [&](Place &a, uint32_t pos, int32_t page) {
+                const uint32_t r = pos & ((1u << p.c.page_shift) - 1);
+                a.row = (uint32_t)page < p.c.n_pages;
+                a.codes = code_off<FMT, HD>(p.c, (uint32_t)page, sg.head, r) + off;
+                a.scales = scale_off<HD>(p.c, (uint32_t)page, sg.head, r);
+            };
+            auto fetch = [&](Codes<FMT, HD> &cd, const uint8_t *codes, const uint8_t *scales, const Place &a) {
+                if (a.row)
+                    cd.load(codes + a.codes, scales + a.scales);
+                else
                     cd.clear();
-                }
             };
 #pragma unroll
-            for (uint32_t i = 0; i < TASKS; ++i) ids[i] = page_of(start + pos0 + 64 * i);
-#pragma unroll
             for (uint32_t i = 0; i < TASKS; ++i) {
-                fetch(kc[i], p.c.k, p.c.ks, start + pos0 + 64 * i, ids[i]);
-                fetch(vc[i], p.c.v, p.c.vs, start + pos0 + 64 * i, ids[i]);
+                place(at[i], start + pos0 + 64 * i, page_of(start + pos0 + 64 * i));
+                fetch(kc[i], p.c.k, p.c.ks, at[i]);
+                fetch(vc[i], p.c.v, p.c.vs, at[i]);
             }
             // ---- query rows: after the previous segment's last S
             if (tile && !(ok = warp_wait(&kempty[(tile - 1) & 1], ((tile - 1) >> 1) & 1))) break;
@@ -1059,7 +1089,8 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
                 for (uint32_t i = 0; i < TASKS; ++i) {
                     kc[i].template store<TN>(ks + st * BG::KV_BYTES, pos0 + 64 * i, pair);
-                    fetch(kc[i], p.c.k, p.c.ks, pos + TN + pos0 + 64 * i, next[i]);
+                    place(at[i], pos + TN + pos0 + 64 * i, next[i]);
+                    fetch(kc[i], p.c.k, p.c.ks, at[i]);
                 }
                 if (id < 32) {  // pages outside the cache: groups of 16 positions
                     const uint32_t at = pos + 16 * lane;
@@ -1078,7 +1109,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
                 for (uint32_t i = 0; i < TASKS; ++i) {
                     vc[i].template store<TN>(vs + st * BG::KV_BYTES, pos0 + 64 * i, pair);
-                    fetch(vc[i], p.c.v, p.c.vs, pos + TN + pos0 + 64 * i, next[i]);
+                    fetch(vc[i], p.c.v, p.c.vs, at[i]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
