@@ -49,6 +49,17 @@ struct AttnParams {
     Job own, prefix;
 };
 
+// The own positions' kernel may run beside the prefix's, which waited for the stream's
+// earlier work: it reads nothing of it, and ends after it, so that the join waits for both.
+__device__ __forceinline__ bool beside(const AttnParams &p, bool prefix) { return !prefix && p.prefix.ctas; }
+__device__ __forceinline__ void begin_kernel(const AttnParams &p, bool prefix) {
+    if (!beside(p, prefix)) pdl_wait();
+    pdl_launch_dependents();
+}
+__device__ __forceinline__ void end_kernel(const AttnParams &p, bool prefix) {
+    if (beside(p, prefix)) pdl_wait();
+}
+
 __device__ __forceinline__ uint32_t seq_len(const Job &j, uint32_t s) {
     return j.lens ? (uint32_t)min(max(j.lens[s], 0), (int32_t)j.max_len) : j.max_len;
 }
@@ -521,7 +532,7 @@ __device__ __forceinline__ void store2<__nv_bfloat16>(__nv_bfloat16 *p, float x,
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
 __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>::MIN_CTAS)
     attn_mx_kernel(const __grid_constant__ AttnParams p, bool prefix) {
-    pdl_launch_dependents();
+    begin_kernel(p, prefix);
     constexpr bool F32 = sizeof(T) == 4;
     using TT = Tile<FMT, HD, NQ, F32>;
     using R = Ring<FMT, HD>;
@@ -705,8 +716,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             }
         }
     }
-    // The own positions' kernel may start beside the prefix's; it ends after it, and the join waits for this one.
-    if (!prefix && p.prefix.ctas) pdl_wait();
+    end_kernel(p, prefix);
 }
 
 // ---------------------------------------------------------------- many rows: tcgen05
@@ -842,7 +852,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
 template <uint32_t FMT, uint32_t HD, typename T>
 __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     attn_mx_tile_kernel(const __grid_constant__ AttnParams p, bool prefix) {
-    pdl_launch_dependents();
     constexpr bool F32 = sizeof(T) == 4;
     using BG = Big<HD, F32>;
     constexpr uint32_t TN = BG::TN, ROWS = 128, GROUPS = TN / 16;
@@ -871,6 +880,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
         tc::tmem_alloc(&tmem_base, BG::COLS);
         tc::tmem_relinquish();
     }
+    begin_kernel(p, prefix);
     const Located loc = locate<BG::THREADS>(job, p.c.n_kv * job.row_tiles, scan, where);
     tc::fence_before_sync();
     __syncthreads();
@@ -916,9 +926,11 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
                 for (uint32_t c = 0; c < CH; ++c) {
                     load(x, half * CH + c);
+                    float mz[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 2)
-                        mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                        mz[i / 2 % 4] = fmaxf(mz[i / 2 % 4], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                    mx = fmaxf(fmaxf(mz[0], mz[1]), fmaxf(mz[2], mz[3]));
                 }
                 halfmax[tile & 1][half][row] = good ? mx : __uint_as_float(0x7FC00000u);
                 meet();
@@ -1037,13 +1049,13 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             struct Place {
                 uint64_t codes, scales;
                 bool row;
-            } at[TASKS];
+            } next[TASKS];
+            int32_t ids[TASKS];
             auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : -1; };
-            auto place = [&](Place &a, uint32_t pos, int32_t page) {
+            auto place = [&](uint32_t pos, int32_t page) {
                 const uint32_t r = pos & ((1u << p.c.page_shift) - 1);
-                a.row = (uint32_t)page < p.c.n_pages;
-                a.codes = code_off<FMT, HD>(p.c, (uint32_t)page, sg.head, r) + off;
-                a.scales = scale_off<HD>(p.c, (uint32_t)page, sg.head, r);
+                return Place{code_off<FMT, HD>(p.c, (uint32_t)page, sg.head, r) + off,
+                             scale_off<HD>(p.c, (uint32_t)page, sg.head, r), (uint32_t)page < p.c.n_pages};
             };
             auto fetch = [&](Codes<FMT, HD> &cd, const uint8_t *codes, const uint8_t *scales, const Place &a) {
                 if (a.row)
@@ -1051,11 +1063,36 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 else
                     cd.clear();
             };
+            // K of tile t (the codes are in kc): the image, and which groups of positions lie in no page
+            auto put_k = [&](uint32_t t, uint32_t pos) {
+                const uint32_t st = t & 1;
+                if (t >= 2 && !warp_wait(&kempty[st], ((t >> 1) - 1) & 1)) return false;
+#pragma unroll
+                for (uint32_t i = 0; i < TASKS; ++i)
+                    kc[i].template store<TN>(ks + st * BG::KV_BYTES, pos0 + 64 * i, pair);
+                if (id < 32) {
+                    const uint32_t at = pos + 16 * lane;
+                    const bool out = lane < GROUPS && at < stop &&
+                                     (uint32_t)table[at >> p.c.page_shift] >= p.c.n_pages;
+                    const uint32_t bits = __ballot_sync(~0u, out);
+                    if (lane == 0) {
+                        bad_groups[t & 3] = bits;
+                        if (bits) raise_device_error(DEVERR_BAD_ARG);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kfull[st]);
+                return true;
+            };
 #pragma unroll
             for (uint32_t i = 0; i < TASKS; ++i) {
-                place(at[i], start + pos0 + 64 * i, page_of(start + pos0 + 64 * i));
-                fetch(kc[i], p.c.k, p.c.ks, at[i]);
-                fetch(vc[i], p.c.v, p.c.vs, at[i]);
+                const uint32_t pos = start + pos0 + 64 * i;
+                const Place first = place(pos, page_of(pos));
+                fetch(kc[i], p.c.k, p.c.ks, first);
+                fetch(vc[i], p.c.v, p.c.vs, first);
+                next[i] = place(pos + TN, page_of(pos + TN));
+                ids[i] = page_of(pos + 2 * TN);
             }
             // ---- query rows: after the previous segment's last S
             if (tile && !(ok = warp_wait(&kempty[(tile - 1) & 1], ((tile - 1) >> 1) & 1))) break;
@@ -1080,36 +1117,29 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                                                ((c & 7) ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
+                // K runs one tile ahead of V, so that S of the next tile does not wait for P V of the last
+            if (!(ok = put_k(tile, start))) break;
+#pragma unroll
+            for (uint32_t i = 0; i < TASKS; ++i) fetch(kc[i], p.c.k, p.c.ks, next[i]);
             for (uint32_t pos = start; pos < stop; pos += TN, ++tile) {
-                const uint32_t st = tile & 1, use = tile >> 1;
-                int32_t next[TASKS];
+                const uint32_t st = tile & 1;
+                Place after[TASKS];
 #pragma unroll
-                for (uint32_t i = 0; i < TASKS; ++i) next[i] = page_of(pos + TN + pos0 + 64 * i);
-                if (use && !(ok = warp_wait(&kempty[st], (use - 1) & 1))) break;
+                for (uint32_t i = 0; i < TASKS; ++i) after[i] = place(pos + 2 * TN + pos0 + 64 * i, ids[i]);
+                if (pos + TN < stop) {
+                    if (!(ok = put_k(tile + 1, pos + TN))) break;
 #pragma unroll
-                for (uint32_t i = 0; i < TASKS; ++i) {
-                    kc[i].template store<TN>(ks + st * BG::KV_BYTES, pos0 + 64 * i, pair);
-                    place(at[i], pos + TN + pos0 + 64 * i, next[i]);
-                    fetch(kc[i], p.c.k, p.c.ks, at[i]);
-                }
-                if (id < 32) {  // pages outside the cache: groups of 16 positions
-                    const uint32_t at = pos + 16 * lane;
-                    const bool out = lane < GROUPS && at < stop &&
-                                     (uint32_t)table[at >> p.c.page_shift] >= p.c.n_pages;
-                    const uint32_t bits = __ballot_sync(~0u, out);
-                    if (lane == 0) {
-                        bad_groups[tile & 3] = bits;
-                        if (bits) raise_device_error(DEVERR_BAD_ARG);
+                    for (uint32_t i = 0; i < TASKS; ++i) {
+                        fetch(kc[i], p.c.k, p.c.ks, after[i]);
+                        ids[i] = page_of(pos + 3 * TN + pos0 + 64 * i);
                     }
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&kfull[st]);
-                if (use && !(ok = warp_wait(&vempty[st], (use - 1) & 1))) break;
+                if (tile >= 2 && !(ok = warp_wait(&vempty[st], ((tile >> 1) - 1) & 1))) break;
 #pragma unroll
                 for (uint32_t i = 0; i < TASKS; ++i) {
                     vc[i].template store<TN>(vs + st * BG::KV_BYTES, pos0 + 64 * i, pair);
-                    fetch(vc[i], p.c.v, p.c.vs, at[i]);
+                    fetch(vc[i], p.c.v, p.c.vs, next[i]);
+                    next[i] = after[i];
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -1180,88 +1210,90 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     __syncthreads();
     tc::fence_after_sync();
     if (warp == 16) tc::tmem_dealloc(tmem, BG::COLS);
-    if (!prefix && p.prefix.ctas) pdl_wait();
+    end_kernel(p, prefix);
 }
 
 // Joins the partial results of one output row: those of the CTAs that shared its
-// segment, and with a prefix those of both jobs.  Four warps take the partials in turn,
-// four loads in flight each; a row that one CTA wrote whole has nothing to join.
+// segment, and with a prefix those of both jobs.  The places of all partials are worked
+// out first, so that four warps can have four loads each in flight; a row that one CTA
+// wrote whole has nothing to join.
 template <uint32_t HD, typename T>
 __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr uint32_t W = 4, V = HD / 32;  // a lane holds V dimensions
+    constexpr uint32_t W = 4, V = HD / 32, U = 4, LIST = 512;  // a lane holds V dimensions
     __shared__ float sm[W], sl[W], so[W][HD];
+    __shared__ const float *ml_of[LIST], *o_of[LIST];
     const uint32_t row = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t token = row / p.n_heads, head = row % p.n_heads, kvh = head / p.group;
     pdl_wait();
-    // partials of each job: the row's slot, or its place in the slots of CTAs ca..cb
-    uint32_t n[2] = {0, 0}, ca[2] = {0, 0};
-    bool one[2] = {false, false};
-    uint64_t total[2] = {0, 0};
+    // partials of each job: the row's slot, or its place in the slots of CTAs first..last
+    uint32_t n = 0, from[2], count[2], in_tile[2];
+    uint64_t total[2];
 #pragma unroll
     for (uint32_t which = 0; which < 2; ++which) {
         const Job &job = which ? p.prefix : p.own;
-        if (!job.ctas) continue;
+        count[which] = 0, from[which] = 0, total[which] = 0;
         const uint32_t seq = which ? 0 : token / p.q_len;
         const uint32_t r = which ? token * p.group + head % p.group : token % p.q_len * p.group + head % p.group;
+        in_tile[which] = job.ctas ? r % job.tile_rows : 0;
+        if (!job.ctas) continue;
         const uint32_t chunks = seq_chunks(job, seq);
         if (chunks == 0) continue;
         total[which] = which ? (uint64_t)seq_cost(job, 0) * p.c.n_kv * job.row_tiles : job.starts[job.n_seq];
-        const uint64_t first = (which ? 0 : job.starts[seq]) +
-                               (uint64_t)(r / job.tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
-        ca[which] = cta_of(first, total[which], job.ctas);
-        n[which] = cta_of(first + chunks - 1, total[which], job.ctas) - ca[which] + 1;
-        one[which] = n[which] == 1;
-        if (one[which] && !job.row_slots) return;  // written whole (without a prefix)
+        const uint64_t at = (which ? 0 : job.starts[seq]) +
+                            (uint64_t)(r / job.tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
+        from[which] = cta_of(at, total[which], job.ctas);
+        count[which] = cta_of(at + chunks - 1, total[which], job.ctas) - from[which] + 1;
+        if (count[which] == 1 && !job.row_slots) return;  // written whole (without a prefix)
+        n += count[which];
     }
     float m = kNoMax, l = 0.0f, o[V];
 #pragma unroll
     for (uint32_t i = 0; i < V; ++i) o[i] = 0.0f;
-    constexpr uint32_t U = 4;
-    for (uint32_t k0 = warp; k0 < n[0] + n[1]; k0 += W * U) {
-        float pm[U], pl[U], po[U][V];
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t k = k0 + u * W;
-            pm[u] = kNoMax, pl[u] = 0.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i) po[u][i] = 0.0f;
-            if (k >= n[0] + n[1]) continue;
-            const uint32_t which = k >= n[0], at = which ? k - n[0] : k;
+    for (uint32_t base = 0; base < n; base += LIST) {
+        const uint32_t here = min(LIST, n - base);
+        if (base) __syncthreads();
+        for (uint32_t i = threadIdx.x; i < here; i += 128) {
+            const uint32_t k = base + i, which = k >= count[0];
             const Job &job = which ? p.prefix : p.own;
-            const float *ml, *src;
-            if (one[which]) {
-                src = job.row_slots + (uint64_t)row * (HD + 2), ml = src + HD;
+            const uint32_t at = which ? k - count[0] : k, cnt = which ? count[1] : count[0];
+            if (cnt == 1) {
+                o_of[i] = job.row_slots + (uint64_t)row * (HD + 2), ml_of[i] = o_of[i] + HD;
             } else {
-                const uint32_t c = ca[which] + at, tr = job.tile_rows;
-                // a CTA without work of its own (more CTAs than cost)
-                if (total[which] < job.ctas && at &&
-                    cta_start(c, total[which], job.ctas) == cta_start(c + 1, total[which], job.ctas))
-                    continue;
-                const uint32_t r = which ? token * p.group + head % p.group : token % p.q_len * p.group + head % p.group;
+                const uint32_t c = (which ? from[1] : from[0]) + at, tr = job.tile_rows, r = which ? in_tile[1] : in_tile[0];
+                const uint64_t tot = which ? total[1] : total[0];
                 const float *slot = job.slots + (uint64_t)(2 * c + (at == 0)) * tr * (HD + 2);
-                ml = slot + 2 * (r % tr), src = slot + 2 * tr + r % tr * HD;
-            }
-            const float2 x = *reinterpret_cast<const float2 *>(ml);
-            pm[u] = x.x, pl[u] = x.y;
-#pragma unroll
-            for (uint32_t i = 0; i < V; i += 2) {
-                const float2 y = *reinterpret_cast<const float2 *>(src + lane * V + i);
-                po[u][i] = y.x, po[u][i + 1] = y.y;
+                // with more CTAs than cost some have no work
+                const bool idle = at && tot < job.ctas && cta_start(c, tot, job.ctas) == cta_start(c + 1, tot, job.ctas);
+                ml_of[i] = idle ? nullptr : slot + 2 * r, o_of[i] = slot + 2 * tr + r * HD;
             }
         }
-        float mn = m;
+        __syncthreads();
+        for (uint32_t k0 = warp; k0 < here; k0 += W * U) {
+            float2 ml[U], po[U][V / 2];
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
-        const float f = exp2f(m - mn);
-        l *= f, m = mn;
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t k = min(k0 + u * W, here - 1);
+                const bool take = k0 + u * W < here && ml_of[k];
+                ml[u] = take ? *reinterpret_cast<const float2 *>(ml_of[k]) : make_float2(kNoMax, 0.0f);
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) o[i] *= f;
+                for (uint32_t i = 0; i < V / 2; ++i)
+                    po[u][i] = take ? reinterpret_cast<const float2 *>(o_of[k])[lane * (V / 2) + i]
+                                    : make_float2(0.0f, 0.0f);
+            }
+            float mn = m;
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const float g = exp2f(pm[u] - mn);
-            l += pl[u] * g;
+            for (uint32_t u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+            const float f = exp2f(m - mn);
+            l *= f, m = mn;
 #pragma unroll
-            for (uint32_t i = 0; i < V; ++i) o[i] += po[u][i] * g;
+            for (uint32_t i = 0; i < V; ++i) o[i] *= f;
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const float g = exp2f(ml[u].x - mn);
+                l += ml[u].y * g;
+#pragma unroll
+                for (uint32_t i = 0; i < V / 2; ++i) o[2 * i] += po[u][i].x * g, o[2 * i + 1] += po[u][i].y * g;
+            }
         }
     }
     if (lane == 0) sm[warp] = m, sl[warp] = l;
@@ -1324,14 +1356,8 @@ int launch_with_smem(const char *who, cudaStream_t st, K kernel, bool (&ready)[6
         if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    // beside the prefix's kernel, which it does not read from
-    const bool beside = !prefix && p.prefix.ctas;
-    if (beside) {
-        const cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(threads), smem, st, p, prefix);
-        if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
-    } else {
-        kernel<<<ctas, threads, smem, st>>>(p, prefix);
-    }
+    const cudaError_t e = launch_pdl(kernel, dim3(ctas), dim3(threads), smem, st, p, prefix);
+    if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
     return check_launch(who);
 }
 
