@@ -245,7 +245,7 @@ FP4X_API int llama_attn_decode_f32q_bf16kv(fp4x_stream_t stream, uint32_t batch,
  * Position t of a sequence is row t % page_size of its page t / page_size; a slot is
  * page * page_size + row.  k and v 16-byte aligned, page_stride a multiple of 16,
  * scales 8-byte aligned, scale_page_stride a multiple of 8; head_dim 64 or 128;
- * page_size 16, 32, 64, 128 or 256; n_pages * page_size < 2^31. */
+ * page_size 16, 32, 64, 128 or 256; n_pages * page_size < 2^31; strides < 2^32. */
 typedef enum { FP4X_MXFP8 = 0, FP4X_MXFP4 = 1 } fp4x_mx_format;
 typedef enum { FP4X_F32 = 0, FP4X_BF16 = 1 } fp4x_dtype;
 typedef struct fp4x_mxkv {

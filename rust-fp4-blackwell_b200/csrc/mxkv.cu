@@ -21,14 +21,16 @@ bool view(const char *who, const fp4x_mxkv *c, Cache &out) {
         return set_error("%s: n_pages * page_size must stay below 2^31", who), false;
     if (!c->k || !c->v || !c->k_scales || !c->v_scales) return set_error("%s: null cache pointer", who), false;
     const uint64_t row = c->format == FMT_FP8 ? hd : hd / 2;
-    if (c->page_stride < row * ps * c->n_kv_heads || c->scale_page_stride < (uint64_t)(hd / 32) * ps * c->n_kv_heads)
+    if (c->page_stride < row * ps * (uint64_t)c->n_kv_heads || c->scale_page_stride < (uint64_t)(hd / 32) * ps * c->n_kv_heads)
         return set_error("%s: pages overlap (strides below one page)", who), false;
+    if (c->page_stride >> 32 || c->scale_page_stride >> 32)
+        return set_error("%s: a page stride must stay below 4 GiB", who), false;
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % 16)
         return set_error("%s: codes and their page stride must be 16-byte aligned", who), false;
     if (!aligned(c->k_scales, 8) || !aligned(c->v_scales, 8) || c->scale_page_stride % 8)
         return set_error("%s: scales and their page stride must be 8-byte aligned", who), false;
     out.k = c->k, out.ks = c->k_scales, out.v = c->v, out.vs = c->v_scales;
-    out.page_stride = c->page_stride, out.scale_stride = c->scale_page_stride;
+    out.page_stride = (uint32_t)c->page_stride, out.scale_stride = (uint32_t)c->scale_page_stride;
     out.n_pages = c->n_pages, out.n_kv = c->n_kv_heads;
     out.page_shift = 31 - __builtin_clz(ps);
     return true;

@@ -9,10 +9,12 @@ namespace mxkv {
 
 enum : uint32_t { FMT_FP8 = FP4X_MXFP8, FMT_FP4 = FP4X_MXFP4 };
 
-// Device view of a cache.  Offsets stay 64-bit: a pool of long contexts passes 4 GB.
+// Device view of a cache.  Offsets into it are 64-bit (a pool of long contexts passes
+// 4 GB), those within a page 32-bit: one widening multiply-add makes an address, where
+// 64-bit strides took a fifth of the attention kernels' instructions.
 struct Cache {
     uint8_t *k, *ks, *v, *vs;
-    uint64_t page_stride, scale_stride;  // bytes between pages
+    uint32_t page_stride, scale_stride;  // bytes between pages
     uint32_t n_pages, page_shift, n_kv;
 };
 
@@ -27,11 +29,11 @@ struct Row {
 // Byte offsets of (page, head, row in page).
 template <uint32_t FMT, uint32_t HD>
 __device__ __forceinline__ uint64_t code_off(const Cache &c, uint32_t page, uint32_t head, uint32_t row) {
-    return (uint64_t)page * c.page_stride + (((uint64_t)head << c.page_shift) + row) * Row<FMT, HD>::BYTES;
+    return (uint64_t)page * c.page_stride + ((head << c.page_shift) + row) * Row<FMT, HD>::BYTES;
 }
 template <uint32_t HD>
 __device__ __forceinline__ uint64_t scale_off(const Cache &c, uint32_t page, uint32_t head, uint32_t row) {
-    return (uint64_t)page * c.scale_stride + (((uint64_t)head << c.page_shift) + row) * (HD / 32);
+    return (uint64_t)page * c.scale_stride + ((head << c.page_shift) + row) * (HD / 32);
 }
 
 // Checks `c` and fills the device view; a message and false if it is not valid.

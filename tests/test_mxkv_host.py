@@ -18,7 +18,7 @@ def _cache(**kw):
 BAD_CACHES = [dict(page_size=48), dict(page_size=8), dict(head_dim=96), dict(format=2), dict(n_pages=0),
               dict(n_kv_heads=0), dict(k=None), dict(v_scales=None), dict(k=4104), dict(page_stride=64 * 8 * 128 - 16),
               dict(page_stride=64 * 8 * 128 + 8), dict(scale_page_stride=64 * 8 * 4 - 8), dict(k_scales=8196),
-              dict(scale_page_stride=64 * 8 * 4 + 4), dict(n_pages=1 << 25)]
+              dict(scale_page_stride=64 * 8 * 4 + 4), dict(n_pages=1 << 25), dict(page_stride=1 << 32), dict(scale_page_stride=1 << 32)]
 
 
 def _p(c):
