@@ -9,10 +9,13 @@
 // attn_mx_kernel streams codes: a warp owns 16-position tiles, copies each lane's own
 // codes with cp.async into a ring only that lane reads (no barrier in the loop), and
 // contracts on mma.m16n8k16 f16 with the query rows as the 8 columns:
-//   S^T = K q^T   in f16 per 32-block, times the block's K scale in f32;
+//   S^T = K q^T   per 32-block, times the block's K scale in f32: in f16, or for MXFP8
+//                 and bf16 queries on the codes as they are, with q as two E4M3 terms
+//                 (to 2^-17 of a row's maximum; values down to 2^-9 of it are exact),
+//                 which needs no conversion;
 //   O^T += V^T P^T in bf16 with the V scale of (position, block) multiplied into P^T.
 // Codes are exact in f16 and bf16 and scales are powers of two, so the only roundings
-// are P to two bf16 terms (16 bits; bf16 queries are exact in f16), or q to an f16 pair
+// are P to two bf16 terms (16 bits; for bf16 queries), or q to an f16 pair
 // and P to three bf16 terms (f32 queries: 22 and 24 bits).  P takes bf16, not f16: its
 // products with the scales, and probabilities far below the maximum, need the range (a
 // dimension in which the largest position's code is 0 is made of those alone).
@@ -25,7 +28,7 @@ namespace mxkv {
 constexpr uint32_t kWarps = 8;                 // warps per CTA
 constexpr uint32_t kChunk = 16 * kWarps;       // positions of one step of a CTA
 constexpr float kNoMax = -3.0e38f;             // running maximum before the first score
-constexpr float kLag = 8.0f;                   // how far (in powers of two) a score may pass the running maximum
+constexpr float kLag = 16.0f;                  // how far (in powers of two) a score may pass the running maximum
 
 // One set of rows over one set of pages: the sequences of a batch over their own
 // pages (n_seq = batch), or all rows of the batch over the shared prefix (n_seq = 1).
@@ -135,6 +138,7 @@ struct Segment {
 struct Segments {
     uint64_t at, end, seq_first;
     uint32_t seq, per;
+    Segments() = default;
     __device__ __forceinline__ Segments(const Job &j, uint32_t n_kv, const Located &loc) {
         at = cta_start(blockIdx.x, loc.total, j.ctas), end = cta_start(blockIdx.x + 1, loc.total, j.ctas);
         seq_first = loc.first, seq = loc.seq, per = n_kv * j.row_tiles;
@@ -207,6 +211,14 @@ __device__ __forceinline__ void e8m0x4_to_bf16(uint32_t w, uint32_t &lo, uint32_
         : "=r"(lo), "=r"(hi)
         : "r"(w));
 }
+// D += A(16x32 E4M3, row) * B(32x8 E4M3, col), f32 accumulate (to 2^-22 of the sum of magnitudes, measured).
+__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // Two E8M0 bytes (in the low half of w) -> two f32.
 __device__ __forceinline__ void e8m0x2_to_f32(uint32_t w, float &lo, float &hi) {
     uint32_t y;
@@ -262,8 +274,13 @@ template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
 struct Tile {
     using R = Ring<FMT, HD>;
     static constexpr uint32_t NB = HD / 32, MT = HD / 16, CW = R::CW, TERMS = F32 ? 2 : 1, PTERMS = F32 ? 3 : 2;
+    // K codes straight into m16n8k32 E4M3 MMAs (a 32-block each, 1.9 times the rate of the two f16 MMAs of 16)
+    static constexpr bool QK8 = false;
     static constexpr bool QREG = NQ == 1 && !F32;
-    static constexpr uint32_t Q_BYTES = TERMS * 2 * NB * NQ * 32 * 8;  // [term][half][block][column tile][lane] 8 B
+    // f16: [term][half][block][column tile][lane], E4M3: [term][block][column tile][lane]; 8 bytes each
+    static constexpr uint32_t Q_BYTES = TERMS * 2 * NB * NQ * 32 * 8;
+    // queries are scaled to a maximum in [2^Q_TOP, 2^(Q_TOP + 1)); E4M3 ends at 1.75 * 2^8
+    static constexpr int Q_TOP = QK8 ? 7 : 14;
     static constexpr uint32_t MERGE_BYTES = kWarps * MT * 32 * 16;
     static constexpr uint32_t SMEM = kWarps * R::STAGES * R::STAGE + Q_BYTES + MERGE_BYTES;
     static constexpr uint32_t MIN_CTAS = NQ * HD <= 128 ? 2 : 1;
@@ -358,7 +375,7 @@ __device__ __forceinline__ void value_fragments(const uint32_t (&vw)[4][Ring<FMT
 }
 
 // One tile from the ring into the running softmax.  `left` positions of the tile
-// exist (0: a page outside the cache); lim[n][j] - first is the column's limit.
+// exist (0: a page outside the cache); lim[8 n + j] is the limit of column 2 t + j of tile n.
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
 __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ring, uint32_t qs, uint32_t left,
                                           bool masked, const int32_t *lim, int32_t first, const float *rf,
@@ -402,35 +419,53 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
         }
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            uint32_t a[2][4];
+            if constexpr (TT::QK8) {
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
+                for (uint32_t n = 0; n < NQ; ++n) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    if constexpr (FMT == FMT_FP8) {
-                        e4m3x4_to_f16(kw[i][h * CW + b], a[h][i], a[h][2 + i]);
-                    } else {
-                        uint32_t f[4];
-                        decode_word_f16(kw[i][h * CW + b / 2], f);
-                        a[h][i] = f[2 * (b & 1)], a[h][2 + i] = f[2 * (b & 1) + 1];
-                    }
-                }
-#pragma unroll
-            for (uint32_t n = 0; n < NQ; ++n) {
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (uint32_t z = 0; z < TERMS; ++z)
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
+                    for (uint32_t z = 0; z < 2; ++z) {
                         uint32_t qf[2];
                         if constexpr (TT::QREG)
-                            qf[0] = T.q[h * NB + b].x, qf[1] = T.q[h * NB + b].y;
+                            qf[0] = T.q[z * NB + b].x, qf[1] = T.q[z * NB + b].y;
                         else
-                            lds_words<2>(qs + ((((z * 2 + h) * NB + b) * NQ + n) * 32 + lane) * 8, qf);
-                        mma_f16_16816(acc, a[h], qf[0], qf[1], acc);
+                            lds_words<2>(qs + (((z * NB + b) * NQ + n) * 32 + lane) * 8, qf);
+                        mma_e4m3_16832(acc, kw[0][b], kw[1][b], kw[0][CW + b], kw[1][CW + b], qf[0], qf[1]);
                     }
-                s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
-                s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
+                    s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
+                    s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
+                }
+            } else {
+                uint32_t a[2][4];
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        if constexpr (FMT == FMT_FP8) {
+                            e4m3x4_to_f16(kw[i][h * CW + b], a[h][i], a[h][2 + i]);
+                        } else {
+                            uint32_t f[4];
+                            decode_word_f16(kw[i][h * CW + b / 2], f);
+                            a[h][i] = f[2 * (b & 1)], a[h][2 + i] = f[2 * (b & 1) + 1];
+                        }
+                    }
+#pragma unroll
+                for (uint32_t n = 0; n < NQ; ++n) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (uint32_t z = 0; z < TERMS; ++z)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            uint32_t qf[2];
+                            if constexpr (TT::QREG)
+                                qf[0] = T.q[h * NB + b].x, qf[1] = T.q[h * NB + b].y;
+                            else
+                                lds_words<2>(qs + ((((z * 2 + h) * NB + b) * NQ + n) * 32 + lane) * 8, qf);
+                            mma_f16_16816(acc, a[h], qf[0], qf[1], acc);
+                        }
+                    s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
+                    s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
+                }
             }
         }
     }
@@ -443,7 +478,7 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
             s[n][j] *= rf[n * 2 + (j & 1)];
             if (masked) {
                 const int32_t pos = (int32_t)(g + 8 * (j / 2));
-                if (pos >= (int32_t)left || first + pos >= lim[n * 2 + (j & 1)]) s[n][j] = -INFINITY;
+                if (pos >= (int32_t)left || first + pos >= lim[n * 8 + (j & 1)]) s[n][j] = -INFINITY;
             }
             above |= s[n][j] > T.m[n][j & 1] + kLag;
         }
@@ -548,52 +583,65 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
     uint8_t *qbuf = smem + kWarps * R::STAGES * R::STAGE;
     float4 *merge = reinterpret_cast<float4 *>(qbuf + TT::Q_BYTES);
     const Located loc = locate<kWarps * 32>(job, p.c.n_kv * job.row_tiles, scan, where);
-    Segments segments(job, p.c.n_kv, loc);
-    // The segment in work, as this warp sees it: its tiles are c * kWarps + warp for c in
-    // [c0, c1), those that start below len.
-    Segment sg = {};
-    uint32_t n_tiles = 0, bad = 0;  // bit s of bad: the page of the tile in stage s is outside the cache
-    int32_t ids = 0;                // lane j: page of tile (j modulo 32)
+    // The walk over the segments lives in shared memory, one copy per warp: its state
+    // would hold some thirty registers through the loop over the tiles.
+    __shared__ Segments walk[kWarps];
+    __shared__ Segment segs[kWarps][2];
+    if (lane == 0) walk[warp] = Segments(job, p.c.n_kv, loc);
+    __syncwarp();
+    // The segment that copies are issued for: this warp's tiles are c * kWarps + warp for
+    // c in [c0, c1), those that start below len.
+    uint32_t c0 = 0, len = 0, head = 0, n_tiles = 0;
+    uint32_t bad = 0;  // bit s: the page of the tile in stage s is outside the cache
+    int32_t ids = 0;   // lane j: page of tile (j modulo 32)
     const int32_t *table = nullptr;
     auto issue = [&](uint32_t j) {
         if (j < n_tiles) {
-            if ((j & 31) == 0) ids = j + lane < n_tiles ? table[((sg.c0 + j + lane) * kWarps + warp) * 16 >> p.c.page_shift] : 0;
-            const uint32_t first = ((sg.c0 + j) * kWarps + warp) * 16;
+            if ((j & 31) == 0) ids = j + lane < n_tiles ? table[((c0 + j + lane) * kWarps + warp) * 16 >> p.c.page_shift] : 0;
+            const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
             const int32_t page = __shfl_sync(~0u, ids, j & 31);
-            issue_tile<FMT, HD>(p.c, ring + j % R::STAGES * R::STAGE, page, sg.head,
-                                first & ((1u << p.c.page_shift) - 1), min(16u, sg.len - first), lane);
+            issue_tile<FMT, HD>(p.c, ring + j % R::STAGES * R::STAGE, page, head,
+                                first & ((1u << p.c.page_shift) - 1), min(16u, len - first), lane);
             const bool out = (uint32_t)page >= p.c.n_pages;
             bad = (bad & ~(1u << j % R::STAGES)) | ((uint32_t)out << j % R::STAGES);
             if (out && lane == 0) raise_device_error(DEVERR_BAD_ARG);
         }
         cp_async_commit();
     };
-    auto open = [&]() {  // the next segment and its first copies
-        if (!segments.next(job, p.c.n_kv, sg)) return false;
+    auto open = [&](uint32_t slot) {  // the next segment and its first copies
+        Segments it = walk[warp];
+        Segment sg = {};
+        const bool any = it.next(job, p.c.n_kv, sg);
+        __syncwarp();
+        if (lane == 0) walk[warp] = it, segs[warp][slot] = sg;
+        __syncwarp();
+        if (!any) return false;
+        c0 = sg.c0, len = sg.len, head = sg.head;
         table = job.pages + (uint64_t)sg.seq * job.table_stride;
-        const uint32_t tiles = (sg.len + 15) / 16;
-        n_tiles = sg.c1 - sg.c0;
-        while (n_tiles && (sg.c0 + n_tiles - 1) * kWarps + warp >= tiles) --n_tiles;
+        const uint32_t tiles = (len + 15) / 16;
+        n_tiles = sg.c1 - c0;
+        while (n_tiles && (c0 + n_tiles - 1) * kWarps + warp >= tiles) --n_tiles;
 #pragma unroll
         for (uint32_t j = 0; j < R::STAGES; ++j) issue(j);
         return true;
     };
-    bool more = open();
-    while (more) {
-        const Segment cur = sg;
-        const uint32_t seq = cur.seq, len = cur.len, head = cur.head, r0 = cur.r0, rows = cur.rows, c0 = cur.c0;
-        // ---- query rows: scaled to a maximum in [2^14, 2^15), f16 (and the remainder's f16), fragment order
+    uint32_t slot_of = 0;
+    for (bool more = open(0); more;) {
+        const Segment &cur = segs[warp][slot_of];
+        slot_of ^= 1;
+        // ---- query rows: scaled by a power of two, in terms, fragment order
         for (uint32_t r = warp; r < ROWS; r += kWarps) {
             float x[HD / 32], amax = 0.0f;
-            const RowAt ra = row_at(p, prefix, seq, head, r0 + min(r, rows - 1));
+            const RowAt ra = row_at(p, prefix, cur.seq, cur.head, cur.r0 + min(r, cur.rows - 1));
             const T *src = (const T *)p.q + (uint64_t)ra.token * p.q_stride + ra.head * HD;
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b) x[b] = r < rows ? (float)src[b * 32 + lane] : 0.0f, amax = fmaxf(amax, fabsf(x[b]));
+            for (uint32_t b = 0; b < NB; ++b) x[b] = r < cur.rows ? (float)src[b * 32 + lane] : 0.0f, amax = fmaxf(amax, fabsf(x[b]));
             amax = warp_max(amax);
             const int e = amax > 0.0f ? max(-112, min(127, (int)(__float_as_uint(amax) >> 23) - 127)) : 0;
-            const float up = pow2(14 - e);
+            const int up_by = TT::Q_TOP - e + (TT::QK8 && (__float_as_uint(amax) & 0x7FFFFFu) <= 0x600000u);
+            const float up = pow2(up_by);
             if (lane == 0) {
-                rowf[r] = p.scale * pow2(max(e - 14, -126));
+                rowf[r] = p.scale * pow2(max(-up_by, -126));
                 limit[r] = prefix ? (int32_t)len
                                   : (int32_t)len - (int32_t)p.q_len + 1 + (int32_t)ra.step;
             }
@@ -603,6 +651,15 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
                 const uint32_t c = lane >> 2, i = lane & 3;
                 const uint32_t tt = R::PAIR ? c / 2 : c & 3, h = R::PAIR ? c & 1 : c >> 2;
                 float y = x[b] * up;
+                if constexpr (TT::QK8) {
+#pragma unroll
+                    for (uint32_t z = 0; z < 2; ++z) {
+                        const uint32_t code = e4m3x2(y, 0.0f) & 0xFF;
+                        const uint32_t back = e4m3x2_to_f16x2(code);
+                        y -= __low2float(*reinterpret_cast<const __half2 *>(&back));
+                        qbuf[(((z * NB + b) * NQ + r / 8) * 32 + (r % 8) * 4 + tt) * 8 + h * 4 + i] = (uint8_t)code;
+                    }
+                } else
 #pragma unroll
                 for (uint32_t z = 0; z < TT::TERMS; ++z) {
                     const __half hy = __float2half_rn(y);
@@ -616,14 +673,13 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         TT tile;
         tile.reset();
         float rf[2 * NQ];
-        int32_t lim[2 * NQ], lowest = 0x7FFFFFFF;
+        int32_t lowest = 0x7FFFFFFF;
 #pragma unroll
         for (uint32_t n = 0; n < NQ; ++n)
 #pragma unroll
             for (uint32_t j = 0; j < 2; ++j) {
                 rf[n * 2 + j] = rowf[n * 8 + 2 * t + j];
-                lim[n * 2 + j] = limit[n * 8 + 2 * t + j];
-                lowest = min(lowest, lim[n * 2 + j]);
+                lowest = min(lowest, limit[n * 8 + 2 * t + j]);
             }
         lowest = min(lowest, __shfl_xor_sync(~0u, lowest, 1));
         lowest = min(lowest, __shfl_xor_sync(~0u, lowest, 2));
@@ -638,12 +694,12 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             uint32_t left = min(16u, len - first);
             bool masked = (int32_t)(first + 16) > lowest || left < 16;
             if ((bad >> stage) & 1) left = 0, masked = true;
-            take_tile<FMT, HD, NQ, F32>(tile, ring + stage * R::STAGE, smem_u32(qbuf), left, masked, lim,
+            take_tile<FMT, HD, NQ, F32>(tile, ring + stage * R::STAGE, smem_u32(qbuf), left, masked, limit + 2 * t,
                                         (int32_t)first, rf, lane);
             stage = stage + 1 == R::STAGES ? 0 : stage + 1;
             issue(j + R::STAGES);
         }
-        more = open();  // its first copies run under the joining of this one
+        more = open(slot_of);  // its first copies run under the joining of this one
         // ---- join the warps
 #pragma unroll
         for (uint32_t n = 0; n < NQ; ++n)
@@ -668,11 +724,11 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         const bool whole = cur.whole();
         float *slot = nullptr;
         if (!whole) {
-            slot = job.slots + (uint64_t)(2 * blockIdx.x + (c0 == 0)) * ROWS * (HD + 2);
+            slot = job.slots + (uint64_t)(2 * blockIdx.x + (cur.c0 == 0)) * ROWS * (HD + 2);
             if (threadIdx.x < ROWS) slot[2 * threadIdx.x] = top[threadIdx.x], slot[2 * threadIdx.x + 1] = sum[threadIdx.x];
             slot += 2 * ROWS;
-        } else if (job.row_slots && threadIdx.x < rows) {
-            const RowAt ra = row_at(p, prefix, seq, head, r0 + threadIdx.x);
+        } else if (job.row_slots && threadIdx.x < cur.rows) {
+            const RowAt ra = row_at(p, prefix, cur.seq, cur.head, cur.r0 + threadIdx.x);
             float *rs = job.row_slots + ((uint64_t)ra.token * p.n_heads + ra.head) * (HD + 2);
             rs[HD] = top[threadIdx.x], rs[HD + 1] = sum[threadIdx.x];
         }
@@ -698,13 +754,13 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
                     const uint32_t r = n * 8 + 2 * t + j;
-                    if (r >= rows) continue;
+                    if (r >= cur.rows) continue;
                     const float y0 = j ? acc.y : acc.x, y1 = j ? acc.w : acc.z;
                     if (!whole) {
                         store2<float>(slot + r * HD + d, y0, y1);
                         continue;
                     }
-                    const RowAt ra = row_at(p, prefix, seq, head, r0 + r);
+                    const RowAt ra = row_at(p, prefix, cur.seq, cur.head, cur.r0 + r);
                     const uint64_t row = (uint64_t)ra.token * p.n_heads + ra.head;
                     if (job.row_slots) {
                         store2<float>(job.row_slots + row * (HD + 2) + d, y0, y1);
