@@ -6,9 +6,9 @@
 //   s_t = q . k_t / sqrt(hd),  out = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),
 // one pass with a running maximum m and sum; partial results join as (m, l, o).
 //
-// attn_mx_kernel streams codes: a warp owns 16-position tiles, copies each lane's own
-// codes with cp.async into a ring only that lane reads (no barrier in the loop), and
-// contracts on mma.m16n8k16 f16 with the query rows as the 8 columns:
+// attn_mx_kernel streams codes: a warp owns 16-position tiles, copies them with cp.async
+// into a ring of its own (no barrier of the CTA in the loop), and contracts on mma.sync
+// with the query rows as the 8 columns:
 //   S^T = K q^T   per 32-block, times the block's K scale in f32: in f16, or for MXFP8
 //                 and bf16 queries on the codes as they are, with q as two E4M3 terms
 //                 (to 2^-17 of a row's maximum; values down to 2^-9 of it are exact),
@@ -251,23 +251,28 @@ __device__ __forceinline__ float pow2(int e) {  // 2^e, -126 <= e <= 127
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// Shapes of the streaming kernel's ring.  A tile is 16 positions; lane (g, t) copies
-//   K: positions g and g + 8, the two chunks of each that hold its columns (t and t + 4,
-//      or 2t and 2t + 1 where two chunks make one 16- or 8-byte copy);
-//   V: positions 2t, 2t + 1, 2t + 8, 2t + 9, chunk g;
-//   the scales of those positions.
+// The streaming kernel's ring.  A tile is 16 positions: their K codes, V codes and
+// scales are four contiguous pieces of a page, copied 16 (scales: 8) bytes per lane in
+// address order.  (Copied by the lanes that use them, V's pieces asked the L2 for single
+// sectors, and the kernel stopped at 5.0 TB/s with all arithmetic taken out.)  Lane
+// (g, t) uses
+//   K: positions g and g + 8, two chunks of each: t and t + 4, or 2t and 2t + 1 where two
+//      chunks make one 16- or 8-byte load;
+//   V: positions 2t, 2t + 1, 2t + 8, 2t + 9, chunk g.
+// at() places a row's 16-byte pieces so that both kinds of loads touch every bank once.
 template <uint32_t FMT, uint32_t HD>
 struct Ring {
-    static constexpr uint32_t NB = HD / 32, CHUNK = Row<FMT, HD>::CHUNK, CW = CHUNK / 4;
-    static constexpr bool PAIR = CHUNK < 16;  // both K chunks of a position in one copy
-    static constexpr uint32_t KCOPY = PAIR ? 2 * CHUNK : CHUNK, KN = PAIR ? 2 : 4;
-    static constexpr uint32_t VS = 2 * NB;    // bytes of two positions' V scales
-    static constexpr uint32_t LANE = KN * KCOPY + 4 * CHUNK + 2 * 4 + 2 * VS;
-    static constexpr uint32_t STAGE = 32 * LANE;
-    static constexpr uint32_t K_OFF = 0, V_OFF = 32 * KN * KCOPY, VS_OFF = V_OFF + 32 * 4 * CHUNK,
-                              KS_OFF = VS_OFF + 32 * 2 * VS;
+    static constexpr uint32_t NB = HD / 32, B = Row<FMT, HD>::BYTES, CHUNK = Row<FMT, HD>::CHUNK, CW = CHUNK / 4;
+    static constexpr bool PAIR = CHUNK < 16;  // both K chunks of a position in one load
+    static constexpr uint32_t K_OFF = 0, V_OFF = 16 * B, KS_OFF = 32 * B, VS_OFF = KS_OFF + 16 * NB;
+    static constexpr uint32_t STAGE = VS_OFF + 16 * NB;
     // two CTAs per SM share 227 KB with their 16 or 32 KB merge buffers
     static constexpr uint32_t STAGES = STAGE > 3000 ? 2 : STAGE > 2000 ? 3 : 4;
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
+        if (B == 128) return row * B + ((piece ^ (row & 6) ^ ((row & 1) << 2)) << 4);
+        const uint32_t slot = row ^ ((row >> 2) & 1);
+        return slot * B + ((B == 64 ? piece ^ (row & 2) : piece) << 4);
+    }
 };
 
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
@@ -305,32 +310,22 @@ template <uint32_t FMT, uint32_t HD>
 __device__ __forceinline__ void issue_tile(const Cache &c, uint32_t ring, int32_t page, uint32_t head, uint32_t row0,
                                            uint32_t left, uint32_t lane) {
     using R = Ring<FMT, HD>;
-    constexpr uint32_t B = Row<FMT, HD>::BYTES, NB = HD / 32;
-    const uint32_t g = lane >> 2, t = lane & 3;
+    constexpr uint32_t NB = HD / 32, PIECES = R::B / 16;  // of a row
     const bool ok = (uint32_t)page < c.n_pages;
     const uint32_t p = ok ? (uint32_t)page : 0;
     const uint32_t n = ok ? left : 0;  // positions of the tile that exist
-    const uint64_t co = code_off<FMT, HD>(c, p, head, row0), so = scale_off<HD>(c, p, head, row0);
-    const uint8_t *k = c.k + co, *v = c.v + co, *ks = c.ks + so, *vs = c.vs + so;
+    const uint64_t co = code_off<FMT, HD>(c, p, head, row0) + lane * 16, so = scale_off<HD>(c, p, head, row0);
+    const uint8_t *k = c.k + co, *v = c.v + co;
 #pragma unroll
-    for (uint32_t i = 0; i < R::KN; ++i) {
-        const uint32_t pos = g + 8 * (R::PAIR ? i : i / 2);
-        const uint32_t off = R::PAIR ? t * R::KCOPY : (t + 4 * (i & 1)) * R::CHUNK;
-        cp_async(ring + R::K_OFF + (i * 32 + lane) * R::KCOPY, k + pos * B + off, R::KCOPY, n ? R::KCOPY : 0);
+    for (uint32_t i = 0; i < PIECES / 2; ++i) {
+        const uint32_t x = i * 32 + lane, row = x / PIECES, dst = ring + R::at(row, x % PIECES);
+        cp_async(dst + R::K_OFF, k + i * 512, 16, n ? 16 : 0);
+        cp_async(dst + R::V_OFF, v + i * 512, 16, row < n ? 16 : 0);  // V of positions that do not exist: zeros
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t pos = 2 * t + (i & 1) + 8 * (i / 2);
-        cp_async(ring + R::V_OFF + (i * 32 + lane) * R::CHUNK, v + pos * B + g * R::CHUNK, R::CHUNK,
-                 pos < n ? R::CHUNK : 0);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-        const uint32_t pos = 2 * t + 8 * i;
-        cp_async(ring + R::VS_OFF + (i * 32 + lane) * R::VS, vs + pos * NB, R::VS,
-                 pos < n ? min(n - pos, 2u) * NB : 0);
-        const uint32_t kp = (g + 8 * i) * NB & ~3u;  // 64-wide heads: the two rows of a 4-byte piece
-        cp_async(ring + R::KS_OFF + (i * 32 + lane) * 4, ks + kp, 4, n ? 4 : 0);
+    constexpr uint32_t PER = 16 * NB / 8;  // 8-byte pieces of the tile's K (and of its V) scales
+    if (lane < 2 * PER) {
+        const uint32_t x = lane % PER * 8, have = lane < PER ? (n ? 8 : 0) : min(8u, n * NB - min(n * NB, x));
+        cp_async(ring + R::KS_OFF + lane * 8, (lane < PER ? c.ks : c.vs) + so + x, 8, have);
     }
 }
 
@@ -383,7 +378,7 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
     using R = Ring<FMT, HD>;
     using TT = Tile<FMT, HD, NQ, F32>;
     constexpr uint32_t NB = HD / 32, CW = R::CW, TERMS = TT::TERMS;
-    const uint32_t g = lane >> 2;
+    const uint32_t g = lane >> 2, t = lane & 3;
     // ---- S^T = K q^T
     float s[NQ][4];
 #pragma unroll
@@ -392,21 +387,24 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
         for (uint32_t j = 0; j < 4; ++j) s[n][j] = 0.0f;
     {
         uint32_t kw[2][2 * CW];  // [position g, g + 8][chunk half][word]
-        if constexpr (R::PAIR) {
-            lds_words<2 * CW>(ring + R::K_OFF + lane * R::KCOPY, kw[0]);
-            lds_words<2 * CW>(ring + R::K_OFF + (32 + lane) * R::KCOPY, kw[1]);
-        } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                uint32_t w[CW];
-                lds_words<CW>(ring + R::K_OFF + (i * 32 + lane) * R::KCOPY, w);
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t row = g + 8 * i;
+            if constexpr (R::PAIR) {
+                lds_words<2 * CW>(ring + R::K_OFF + R::at(row, t * CW / 2) + t * CW * 8 % 16, kw[i]);
+            } else {
 #pragma unroll
-                for (uint32_t j = 0; j < CW; ++j) kw[i / 2][(i & 1) * CW + j] = w[j];
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t w[CW];
+                    lds_words<CW>(ring + R::K_OFF + R::at(row, t + 4 * h), w);
+#pragma unroll
+                    for (uint32_t j = 0; j < CW; ++j) kw[i][h * CW + j] = w[j];
+                }
             }
         }
-        uint32_t sc[2][1];
-        lds_words<1>(ring + R::KS_OFF + lane * 4, sc[0]);
-        lds_words<1>(ring + R::KS_OFF + (32 + lane) * 4, sc[1]);
+        uint32_t sc[2][1];  // 64-wide heads: the word of two rows
+        lds_words<1>(ring + R::KS_OFF + (g * NB & ~3u), sc[0]);
+        lds_words<1>(ring + R::KS_OFF + ((g + 8) * NB & ~3u), sc[1]);
         float ks[2][NB];
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
@@ -520,14 +518,17 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
     // ---- O^T += V^T (P scaled)^T
     uint32_t vw[4][CW], sc[2][NB];  // scales of positions (2t, 2t + 1) and (2t + 8, 2t + 9) as bf16 pairs
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) lds_words<CW>(ring + R::V_OFF + (i * 32 + lane) * R::CHUNK, vw[i]);
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = 2 * t + (i & 1) + 8 * (i / 2);
+        lds_words<CW>(ring + R::V_OFF + R::at(row, g * R::CHUNK / 16) + g * R::CHUNK % 16, vw[i]);
+    }
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-        uint32_t w[R::VS / 4];
-        lds_words<R::VS / 4>(ring + R::VS_OFF + (i * 32 + lane) * R::VS, w);
-        e8m0x4_to_bf16(NB == 4 ? __byte_perm(w[0], w[R::VS / 4 - 1], 0x5140) : __byte_perm(w[0], 0, 0x3120), sc[i][0],
+        uint32_t w[NB / 2];
+        lds_words<NB / 2>(ring + R::VS_OFF + (2 * t + 8 * i) * NB, w);
+        e8m0x4_to_bf16(NB == 4 ? __byte_perm(w[0], w[NB / 2 - 1], 0x5140) : __byte_perm(w[0], 0, 0x3120), sc[i][0],
                        sc[i][1]);
-        if constexpr (NB == 4) e8m0x4_to_bf16(__byte_perm(w[0], w[R::VS / 4 - 1], 0x7362), sc[i][2], sc[i][3]);
+        if constexpr (NB == 4) e8m0x4_to_bf16(__byte_perm(w[0], w[NB / 2 - 1], 0x7362), sc[i][2], sc[i][3]);
     }
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) {
@@ -691,12 +692,14 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         for (uint32_t j = 0; j < n_tiles; ++j) {
             const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
             cp_async_wait<R::STAGES - 1>();
+            __syncwarp();  // every lane's copies of the tile have landed
             uint32_t left = min(16u, len - first);
             bool masked = (int32_t)(first + 16) > lowest || left < 16;
             if ((bad >> stage) & 1) left = 0, masked = true;
             take_tile<FMT, HD, NQ, F32>(tile, ring + stage * R::STAGE, smem_u32(qbuf), left, masked, limit + 2 * t,
                                         (int32_t)first, rf, lane);
             stage = stage + 1 == R::STAGES ? 0 : stage + 1;
+            __syncwarp();  // every lane has read the stage
             issue(j + R::STAGES);
         }
         more = open(slot_of);  // its first copies run under the joining of this one
