@@ -913,14 +913,15 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     attn_mx_tile_kernel(const __grid_constant__ AttnParams p, bool prefix) {
     constexpr bool F32 = sizeof(T) == 4;
     using BG = Big<HD, F32>;
-    constexpr uint32_t TN = BG::TN, ROWS = 128, GROUPS = TN / 16;
+    constexpr uint32_t TN = BG::TN, ROWS = 128;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t scan[BG::THREADS / 32 + 1];
     __shared__ Located where;
     __shared__ __align__(8) uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pready[2], pvdone[2], done;
-    // bit i: positions 16 i .. of the tile lie in no page.  Four deep: tile t + 4 is written after S of tile t + 2,
-    // which waits for P V of tile t and so for the softmax warps that read tile t's word.
-    __shared__ uint32_t tmem_base, bad_groups[4];
+    // Byte w, bit i: positions 64 i + 8 w .. of the tile lie in no page.  Four deep: tile t + 4 is written after S of
+    // tile t + 2, which waits for P V of tile t and so for the softmax warps that read tile t's bytes.
+    __shared__ __align__(8) uint8_t no_page[4][8];
+    __shared__ uint32_t tmem_base;
     __shared__ float halfmax[2][2][ROWS], halfsum[2][ROWS];
     uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     uint8_t *qs = smem, *ks = smem + BG::Q_BYTES, *vs = ks + 2 * BG::KV_BYTES;
@@ -968,7 +969,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 const uint32_t buf = tile & 1, ph = (tile >> 1) & 1, sb = tmem + lanes + buf * BG::S_COLS;
                 good = good && warp_wait(&sfull[buf], ph);
                 tc::fence_after_sync();
-                const uint32_t bad = *(volatile uint32_t *)&bad_groups[tile & 3];
+                const uint64_t bad = *(volatile uint64_t *)no_page[tile & 3];
                 const bool masked = (int32_t)(pos + TN) > low || bad;
                 const int32_t left = limit - (int32_t)pos;
                 auto load = [&](uint32_t(&x)[32], uint32_t c) {
@@ -976,7 +977,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                     if (masked) {
 #pragma unroll
                         for (uint32_t i = 0; i < 32; ++i)
-                            if ((int32_t)(c * 32 + i) >= left || (bad >> (c * 2 + i / 16)) & 1)
+                            if ((int32_t)(c * 32 + i) >= left || (bad >> ((c % 2 * 4 + i / 8) * 8 + c / 2)) & 1)
                                 x[i] = __float_as_uint(-INFINITY);
                     }
                 };
@@ -1107,14 +1108,16 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             // where a position's row lies, in K and V alike; not in the cache or past the end: no row
             struct Place {
                 uint64_t codes, scales;
-                bool row;
+                bool row, bad;
             } next[TASKS];
+            uint32_t kbad = 0;  // bit i: the positions of kc[i] lie in no page
             int32_t ids[TASKS];
-            auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : -1; };
+            auto page_of = [&](uint32_t pos) { return pos < stop ? table[pos >> p.c.page_shift] : 0; };
             auto place = [&](uint32_t pos, int32_t page) {
                 const uint32_t r = pos & ((1u << p.c.page_shift) - 1);
                 return Place{code_off<FMT, HD>(p.c, (uint32_t)page, sg.head, r) + off,
-                             scale_off<HD>(p.c, (uint32_t)page, sg.head, r), (uint32_t)page < p.c.n_pages};
+                             scale_off<HD>(p.c, (uint32_t)page, sg.head, r), pos < stop && (uint32_t)page < p.c.n_pages,
+                             pos < stop && (uint32_t)page >= p.c.n_pages};
             };
             auto fetch = [&](Codes<FMT, HD> &cd, const uint8_t *codes, const uint8_t *scales, const Place &a) {
                 if (a.row)
@@ -1122,22 +1125,22 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 else
                     cd.clear();
             };
-            // K of tile t (the codes are in kc): the image, and which groups of positions lie in no page
-            auto put_k = [&](uint32_t t, uint32_t pos) {
+            auto fetch_k = [&](const Place(&a)[TASKS]) {
+                kbad = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < TASKS; ++i) fetch(kc[i], p.c.k, p.c.ks, a[i]), kbad |= (uint32_t)a[i].bad << i;
+            };
+            // K of tile t (the codes are in kc): the image, and which positions lie in no page
+            auto put_k = [&](uint32_t t) {
                 const uint32_t st = t & 1;
                 if (t >= 2 && !warp_wait(&kempty[st], ((t >> 1) - 1) & 1)) return false;
 #pragma unroll
                 for (uint32_t i = 0; i < TASKS; ++i)
                     kc[i].template store<TN>(ks + st * BG::KV_BYTES, pos0 + 64 * i, pair);
-                if (id < 32) {
-                    const uint32_t at = pos + 16 * lane;
-                    const bool out = lane < GROUPS && at < stop &&
-                                     (uint32_t)table[at >> p.c.page_shift] >= p.c.n_pages;
-                    const uint32_t bits = __ballot_sync(~0u, out);
-                    if (lane == 0) {
-                        bad_groups[t & 3] = bits;
-                        if (bits) raise_device_error(DEVERR_BAD_ARG);
-                    }
+                const uint32_t bits = __reduce_or_sync(~0u, kbad);
+                if (lane == 0) {
+                    no_page[t & 3][warp - 8] = (uint8_t)bits;
+                    if (bits) raise_device_error(DEVERR_BAD_ARG);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -1147,9 +1150,13 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
             for (uint32_t i = 0; i < TASKS; ++i) {
                 const uint32_t pos = start + pos0 + 64 * i;
-                const Place first = place(pos, page_of(pos));
-                fetch(kc[i], p.c.k, p.c.ks, first);
-                fetch(vc[i], p.c.v, p.c.vs, first);
+                next[i] = place(pos, page_of(pos));
+                fetch(vc[i], p.c.v, p.c.vs, next[i]);
+            }
+            fetch_k(next);
+#pragma unroll
+            for (uint32_t i = 0; i < TASKS; ++i) {
+                const uint32_t pos = start + pos0 + 64 * i;
                 next[i] = place(pos + TN, page_of(pos + TN));
                 ids[i] = page_of(pos + 2 * TN);
             }
@@ -1177,21 +1184,18 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
             }
                 // K runs one tile ahead of V, so that S of the next tile does not wait for P V of the last
-            if (!(ok = put_k(tile, start))) break;
-#pragma unroll
-            for (uint32_t i = 0; i < TASKS; ++i) fetch(kc[i], p.c.k, p.c.ks, next[i]);
+            if (!(ok = put_k(tile))) break;
+            fetch_k(next);
             for (uint32_t pos = start; pos < stop; pos += TN, ++tile) {
                 const uint32_t st = tile & 1;
                 Place after[TASKS];
 #pragma unroll
                 for (uint32_t i = 0; i < TASKS; ++i) after[i] = place(pos + 2 * TN + pos0 + 64 * i, ids[i]);
                 if (pos + TN < stop) {
-                    if (!(ok = put_k(tile + 1, pos + TN))) break;
+                    if (!(ok = put_k(tile + 1))) break;
+                    fetch_k(after);
 #pragma unroll
-                    for (uint32_t i = 0; i < TASKS; ++i) {
-                        fetch(kc[i], p.c.k, p.c.ks, after[i]);
-                        ids[i] = page_of(pos + 3 * TN + pos0 + 64 * i);
-                    }
+                    for (uint32_t i = 0; i < TASKS; ++i) ids[i] = page_of(pos + 3 * TN + pos0 + 64 * i);
                 }
                 if (tile >= 2 && !(ok = warp_wait(&vempty[st], ((tile >> 1) - 1) & 1))) break;
 #pragma unroll
