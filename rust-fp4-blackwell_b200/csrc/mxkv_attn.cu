@@ -288,7 +288,7 @@ struct Tile {
     static constexpr int Q_TOP = QK8 ? 7 : 14;
     static constexpr uint32_t MERGE_BYTES = kWarps * MT * 32 * 16;
     static constexpr uint32_t SMEM = kWarps * R::STAGES * R::STAGE + Q_BYTES + MERGE_BYTES;
-    static constexpr uint32_t MIN_CTAS = NQ * HD <= 128 ? 2 : 1;
+    static constexpr uint32_t MIN_CTAS = NQ * HD <= 256 ? 2 : 1;
 
     float o[MT][NQ][4];
     float m[NQ][2], l[NQ][2];
@@ -1386,7 +1386,7 @@ struct Plan {
     uint64_t own_slots, prefix_slots, row_slots, starts;  // floats
 };
 // CTAs of a job that run at once per SM: see Tile::MIN_CTAS.
-inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows) { return tile_rows * hd <= 1024 ? 2 : 1; }
+inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows) { return tile_rows * hd <= 2048 ? 2 : 1; }
 
 Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uint32_t q_len, uint32_t prefix_len,
                uint32_t max_len) {
@@ -1427,7 +1427,7 @@ int launch_with_smem(const char *who, cudaStream_t st, K kernel, bool (&ready)[6
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
 int launch_stream(const char *who, cudaStream_t st, const AttnParams &p, bool prefix) {
     using TT = Tile<FMT, HD, NQ, sizeof(T) == 4>;
-    static_assert(TT::MIN_CTAS == (8 * NQ * HD <= 1024 ? 2 : 1), "ctas_per_sm and the launch bounds agree");
+    static_assert(TT::MIN_CTAS == (8 * NQ * HD <= 2048 ? 2 : 1), "ctas_per_sm and the launch bounds agree");
     static bool ready[64] = {};
     return launch_with_smem(who, st, attn_mx_kernel<FMT, HD, NQ, T>, ready, (prefix ? p.prefix : p.own).ctas,
                             kWarps * 32, TT::SMEM, p, prefix);

@@ -117,9 +117,8 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_con
     slice_of(p.vocab, p.slices, slice, lo, hi);
     const T *x = (const T *)p.logits + (uint64_t)row * p.stride;
     Stat st{-INFINITY, 0.0f, 0xFFFFFFFFu, 0};
-    constexpr uint32_t U = 4;  // loads in flight per thread
-    for (uint32_t v0 = lo + threadIdx.x * 4; v0 < hi; v0 += kThreads * 4 * U) {
-        float y[U][4];
+    constexpr uint32_t U = 4;  // loads per thread and step; the next step's run under this one's arithmetic
+    auto load = [&](float(&y)[U][4], uint32_t v0) {
 #pragma unroll
         for (uint32_t j = 0; j < U; ++j) {
             const uint32_t v = v0 + j * kThreads * 4;
@@ -130,6 +129,12 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_con
                 for (uint32_t e = 0; e < 4; ++e) y[j][e] = v + e < hi ? load1(x + v + e) : -INFINITY;
             }
         }
+    };
+    float y[U][4], next[U][4];
+    uint32_t v0 = lo + threadIdx.x * 4;
+    load(y, v0);
+    for (; v0 < hi; v0 += kThreads * 4 * U) {
+        load(next, v0 + kThreads * 4 * U);
         float mx = -INFINITY;
 #pragma unroll
         for (uint32_t j = 0; j < U; ++j)
@@ -150,9 +155,13 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_con
 #pragma unroll
             for (uint32_t j = 0; j < U; ++j)
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) s += exp2f((y[j][e] - st.m) * c);
+                for (uint32_t e = 0; e < 4; ++e) s += mxkv::ex2((y[j][e] - st.m) * c);
             st.s += s;
         }
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) y[j][e] = next[j][e];
     }
     st = warp_join(st, c);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = st;
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
                     const uint32_t v = v0 + j * kThreads * 4 + e;
-                    const float w = exp2f((clean(y[j][e]) - st.m) * c) * inv;
+                    const float w = mxkv::ex2((clean(y[j][e]) - st.m) * c) * inv;
                     const float r = v == d ? 0.0f : fmaxf(w - qv[j][e], 0.0f);  // certain drafts: q = 1 at d
                     const float f = __fdividef(1.0f, ev[j][e]);
                     // indices ascend within a thread: a strict comparison keeps the lowest
