@@ -14,6 +14,8 @@
 // moments before, so most of it comes from L2.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "mxkv.cuh"
 
 namespace fp4x {
@@ -24,7 +26,7 @@ constexpr uint32_t kCluster = 8;
 constexpr uint32_t kMaxSlices = 32;  // slices of a row: one lane each when they are joined
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct Stat {  // of a slice or row: max logit, sum of exp((x - max) / T), lowest index of the max
+struct Stat {  // of a slice or row: max logit, sum of exp((x - max) / T), lowest index of the max (greedy)
     float m, s;
     uint32_t i, pad;
 };
@@ -44,31 +46,43 @@ struct Params {
 // NaN -> -inf (fmaxf returns the other operand), +inf -> the largest finite value.
 __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 3.40282347e+38f); }
 
-// Four consecutive values: one 16- or 8-byte load where rows are aligned for it
-// (VEC), else single loads.
-template <bool VEC>
-__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
-    if constexpr (VEC) {
-        const float4 f = __ldg(reinterpret_cast<const float4 *>(p));
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __ldg(p + i);
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float (&x)[4]) {
-    if constexpr (VEC) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-        x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
-        x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
-    }
-}
 __device__ __forceinline__ float load1(const float *p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+
+// Four consecutive values as they were loaded, past `hi` -inf: one 16- or 8-byte load where every row is
+// aligned for it (VEC), else single ones.
+template <typename T, bool VEC>
+struct Raw {
+    using Word = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;
+    Word w;
+    __device__ __forceinline__ void load(const T *x, uint32_t v, uint32_t hi) {
+        if (VEC && v + 4 <= hi) {
+            w = __ldg(reinterpret_cast<const Word *>(x + v));
+            return;
+        }
+        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (v < hi) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (v + e < hi) y[e] = load1(x + v + e);
+        }
+        set(y);
+    }
+    __device__ __forceinline__ void set(const float (&y)[4]) {
+        if constexpr (sizeof(T) == 4)
+            w = make_float4(y[0], y[1], y[2], y[3]);
+        else
+            w = make_uint2(mxkv::pack_bf16x2(y[0], y[1]), mxkv::pack_bf16x2(y[2], y[3]));
+    }
+    __device__ __forceinline__ void get(float (&y)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+            y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+        } else {
+            y[0] = __uint_as_float(w.x << 16), y[1] = __uint_as_float(w.x & 0xFFFF0000u);
+            y[2] = __uint_as_float(w.y << 16), y[3] = __uint_as_float(w.y & 0xFFFF0000u);
+        }
+    }
+};
 
 __device__ __forceinline__ uint32_t drafts_of(const Params &p, uint32_t b) {
     return p.lens ? (uint32_t)min(max(p.lens[b], 0), (int32_t)p.k) : p.k;
@@ -117,51 +131,48 @@ __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_con
     slice_of(p.vocab, p.slices, slice, lo, hi);
     const T *x = (const T *)p.logits + (uint64_t)row * p.stride;
     Stat st{-INFINITY, 0.0f, 0xFFFFFFFFu, 0};
-    constexpr uint32_t U = 4;  // loads per thread and step; the next step's run under this one's arithmetic
-    auto load = [&](float(&y)[U][4], uint32_t v0) {
+    // Two buffers of U loads in turn, kept as loaded until they are used: a conversion or
+    // a move would wait for the data.
+    constexpr uint32_t U = 4, STEP = kThreads * 4 * U;
+    using R = Raw<T, VEC>;
+    auto load = [&](R(&y)[U], uint32_t v0) {
 #pragma unroll
-        for (uint32_t j = 0; j < U; ++j) {
-            const uint32_t v = v0 + j * kThreads * 4;
-            if (v + 4 <= hi) {
-                load4<VEC>(x + v, y[j]);
-            } else {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) y[j][e] = v + e < hi ? load1(x + v + e) : -INFINITY;
-            }
-        }
+        for (uint32_t j = 0; j < U; ++j) y[j].load(x, v0 + j * kThreads * 4, hi);
     };
-    float y[U][4], next[U][4];
-    uint32_t v0 = lo + threadIdx.x * 4;
-    load(y, v0);
-    for (; v0 < hi; v0 += kThreads * 4 * U) {
-        load(next, v0 + kThreads * 4 * U);
-        float mx = -INFINITY;
+    auto take = [&](const R(&raw)[U], uint32_t v0) {
+        float y[U][4], mx = -INFINITY;
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j) raw[j].get(y[j]);
 #pragma unroll
         for (uint32_t j = 0; j < U; ++j)
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) y[j][e] = clean(y[j][e]), mx = fmaxf(mx, y[j][e]);
-        if (mx > st.m) {
-            st.s = st.s * exp2f((st.m - mx) * c), st.m = mx;
-            uint32_t at = 0;  // lowest index that holds the maximum: j ascending, then e
+        if (greedy && mx > st.m) {  // where the maximum is: greedy sequences only, the search costs more than the sum
 #pragma unroll
             for (int j = U - 1; j >= 0; --j)
 #pragma unroll
-                for (int e = 3; e >= 0; --e)
-                    if (y[j][e] == mx) at = v0 + j * kThreads * 4 + e;
-            st.i = at;
+                for (int e = 3; e >= 0; --e)  // downwards: the lowest index stays
+                    if (y[j][e] == mx) st.i = v0 + j * kThreads * 4 + e;
         }
-        if (st.m > -INFINITY) {
-            float s = 0.0f;
+        mx = fmaxf(mx, st.m);
+        if (mx > -INFINITY) {
+            st.s *= mxkv::ex2((st.m - mx) * c), st.m = mx;
+            float s[2] = {0.0f, 0.0f};
 #pragma unroll
             for (uint32_t j = 0; j < U; ++j)
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) s += mxkv::ex2((y[j][e] - st.m) * c);
-            st.s += s;
+                for (uint32_t e = 0; e < 4; ++e) s[e & 1] += mxkv::ex2((y[j][e] - st.m) * c);
+            st.s += s[0] + s[1];
         }
-#pragma unroll
-        for (uint32_t j = 0; j < U; ++j)
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) y[j][e] = next[j][e];
+    };
+    R ya[U], yb[U];
+    uint32_t v0 = lo + threadIdx.x * 4;
+    load(ya, v0);
+    for (; v0 < hi; v0 += 2 * STEP) {
+        load(yb, v0 + STEP);
+        take(ya, v0);
+        load(ya, v0 + 2 * STEP);
+        if (v0 + STEP < hi) take(yb, v0 + STEP);
     }
     st = warp_join(st, c);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = st;
@@ -242,23 +253,22 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
         slice_of(p.vocab, kCluster, rank, lo, hi);
         constexpr uint32_t U = 2;
         for (uint32_t v0 = lo + threadIdx.x * 4; v0 < hi; v0 += kThreads * 4 * U) {
-            float y[U][4], qv[U][4], ev[U][4];
+            Raw<T, VEC> yr[U];
+            Raw<float, VEC> qr[U], er[U];
 #pragma unroll
             for (uint32_t j = 0; j < U; ++j) {
                 const uint32_t v = v0 + j * kThreads * 4;
+                yr[j].load(x, v, hi), er[j].load(noise, v, hi);
+                if (q) qr[j].load(q, v, hi);
+            }
+            float y[U][4], qv[U][4], ev[U][4];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) y[j][e] = -INFINITY, qv[j][e] = 0.0f, ev[j][e] = 1.0f;
-                if (v + 4 <= hi) {
-                    load4<VEC>(x + v, y[j]);
-                    load4<VEC>(noise + v, ev[j]);
-                    if (q) load4<VEC>(q + v, qv[j]);
+            for (uint32_t j = 0; j < U; ++j) {
+                yr[j].get(y[j]), er[j].get(ev[j]);
+                if (q) {
+                    qr[j].get(qv[j]);
                 } else {
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e)
-                        if (v + e < hi) {
-                            y[j][e] = load1(x + v + e), ev[j][e] = noise[v + e];
-                            if (q) qv[j][e] = q[v + e];
-                        }
+                    qv[j][0] = qv[j][1] = qv[j][2] = qv[j][3] = 0.0f;
                 }
             }
 #pragma unroll
@@ -269,8 +279,8 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
                     const float w = mxkv::ex2((clean(y[j][e]) - st.m) * c) * inv;
                     const float r = v == d ? 0.0f : fmaxf(w - qv[j][e], 0.0f);  // certain drafts: q = 1 at d
                     const float f = __fdividef(1.0f, ev[j][e]);
-                    // indices ascend within a thread: a strict comparison keeps the lowest
-                    if (r > 0.0f && r * f > best[0].v) best[0] = Best{r * f, v};
+                    // indices ascend within a thread: a strict comparison keeps the lowest; w is 0 past the row's end
+                    if (w > 0.0f && r * f > best[0].v) best[0] = Best{r * f, v};
                     if (w > 0.0f && w * f > best[1].v) best[1] = Best{w * f, v};
                 }
         }
@@ -292,7 +302,13 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
 #pragma unroll
         for (uint32_t z = 0; z < 2; ++z)
             r[z] = warp_best(lane < kCluster ? *cluster.map_shared_rank(&mine[z], lane) : Best{0.0f, 0xFFFFFFFFu});
-        const uint32_t pick = r[0].i != 0xFFFFFFFFu ? r[0].i : r[1].i != 0xFFFFFFFFu ? r[1].i : st.i;
+        uint32_t pick = r[0].i != 0xFFFFFFFFu ? r[0].i : r[1].i != 0xFFFFFFFFu ? r[1].i : st.i;
+        if (pick >= p.vocab) {  // nothing has any mass: the argmax
+            pick = 0xFFFFFFFFu;
+            for (uint32_t v = lane; v < p.vocab; v += 32)
+                if (clean(load1(x + v)) == st.m) pick = min(pick, v);
+            pick = __reduce_min_sync(~0u, pick);
+        }
         const uint64_t out = (uint64_t)b * (p.k + 1);
         for (uint32_t i = lane; i <= p.k; i += 32) {
             const int32_t tok = i < at ? p.drafts[(uint64_t)b * p.k + i] : i == at ? (int32_t)pick : -1;
@@ -315,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster, 1, 1)
 // Slices per row: enough CTAs for two waves of the 2048-thread SMs, and no slice below
 // 2048 values (its join would cost as much as its reading).
 inline uint32_t slices_of(uint64_t rows, uint32_t vocab) {
-    const uint64_t want = (uint64_t)num_sms() * 16 / (rows ? rows : 1), most = vocab / 2048;
+    const uint64_t want = (uint64_t)num_sms() * 8 / (rows ? rows : 1), most = vocab / 2048;
     const uint64_t n = want < most ? want : most;
     return (uint32_t)(n < 1 ? 1 : n > kMaxSlices ? kMaxSlices : n);
 }
