@@ -130,15 +130,14 @@ __global__ void __launch_bounds__(256) kv_append_kernel(Cache c, uint32_t n, con
                                                         const T *__restrict__ k, uint64_t ks, const T *__restrict__ v,
                                                         uint64_t vs) {
     constexpr uint32_t NB = HD / 32, WORDS = Row<FMT, HD>::CHUNK / 2;
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (uint64_t)n * 2 * c.n_kv * 4) return;  // whole rows of four lanes
-    const RowId<HD> id(i, c.n_kv);
+    // lanes past the end repeat the last row, so that the shuffles run with whole warps
+    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x, total = (uint64_t)n * 2 * c.n_kv * 4;
+    const RowId<HD> id(i < total ? i : total - 4 + (i & 3), c.n_kv);
     const int32_t slot = slots[id.token];
     const T *src = (id.is_v ? v + id.token * vs : k + id.token * ks) + id.head * HD + id.t * 8;
     float x[NB][8];
 #pragma unroll
     for (uint32_t b = 0; b < NB; ++b) load8<T>(src + b * 32, x[b]);
-    const uint32_t mask = 0xFu << (threadIdx.x & 28);
     uint32_t w[WORDS], scales = 0;
 #pragma unroll
     for (uint32_t j = 0; j < WORDS; ++j) w[j] = 0;
@@ -151,8 +150,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(Cache c, uint32_t n, con
             amax = fmaxf(amax, fabsf(x[b][j]));
             if (FMT == FMT_FP4) nan |= x[b][j] != x[b][j];
         }
-        amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(mask, amax, 2));
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
         uint32_t e = e8m0_of(amax, FMT == FMT_FP8 ? 8 : 2);
         float s0, s1;
         inv_scale(e, s0, s1);
@@ -168,10 +167,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(Cache c, uint32_t n, con
                 w[(h * NB + b) / 2] |= half << (16 * (b & 1));
             }
         }
-        if (FMT == FMT_FP4 && __any_sync(mask, nan)) e = 255;
+        if (FMT == FMT_FP4 && (__ballot_sync(~0u, nan) >> (threadIdx.x & 28) & 0xF)) e = 255;
         scales |= e << (8 * b);
     }
-    if (slot < 0) return;
+    if (slot < 0 || i >= total) return;
     const uint32_t page = (uint32_t)slot >> c.page_shift, row = (uint32_t)slot & ((1u << c.page_shift) - 1);
     if (page >= c.n_pages) {
         raise_device_error(DEVERR_BAD_ARG);

@@ -9,13 +9,10 @@
 // attn_mx_kernel streams codes: a warp owns 16-position tiles, copies them with cp.async
 // into a ring of its own (no barrier of the CTA in the loop), and contracts on mma.sync
 // with the query rows as the 8 columns:
-//   S^T = K q^T   per 32-block, times the block's K scale in f32: in f16, or for MXFP8
-//                 and bf16 queries on the codes as they are, with q as two E4M3 terms
-//                 (to 2^-17 of a row's maximum; values down to 2^-9 of it are exact),
-//                 which needs no conversion;
+//   S^T = K q^T   in f16 per 32-block, times the block's K scale in f32;
 //   O^T += V^T P^T in bf16 with the V scale of (position, block) multiplied into P^T.
 // Codes are exact in f16 and bf16 and scales are powers of two, so the only roundings
-// are P to two bf16 terms (16 bits; for bf16 queries), or q to an f16 pair
+// are P to two bf16 terms (16 bits; bf16 queries are exact in f16), or q to an f16 pair
 // and P to three bf16 terms (f32 queries: 22 and 24 bits).  P takes bf16, not f16: its
 // products with the scales, and probabilities far below the maximum, need the range (a
 // dimension in which the largest position's code is 0 is made of those alone).
@@ -211,14 +208,6 @@ __device__ __forceinline__ void e8m0x4_to_bf16(uint32_t w, uint32_t &lo, uint32_
         : "=r"(lo), "=r"(hi)
         : "r"(w));
 }
-// D += A(16x32 E4M3, row) * B(32x8 E4M3, col), f32 accumulate (to 2^-22 of the sum of magnitudes, measured).
-__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // Two E8M0 bytes (in the low half of w) -> two f32.
 __device__ __forceinline__ void e8m0x2_to_f32(uint32_t w, float &lo, float &hi) {
     uint32_t y;
@@ -279,13 +268,9 @@ template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
 struct Tile {
     using R = Ring<FMT, HD>;
     static constexpr uint32_t NB = HD / 32, MT = HD / 16, CW = R::CW, TERMS = F32 ? 2 : 1, PTERMS = F32 ? 3 : 2;
-    // K codes straight into m16n8k32 E4M3 MMAs (a 32-block each, 1.9 times the rate of the two f16 MMAs of 16)
-    static constexpr bool QK8 = false;
     static constexpr bool QREG = NQ == 1 && !F32;
-    // f16: [term][half][block][column tile][lane], E4M3: [term][block][column tile][lane]; 8 bytes each
-    static constexpr uint32_t Q_BYTES = TERMS * 2 * NB * NQ * 32 * 8;
-    // queries are scaled to a maximum in [2^Q_TOP, 2^(Q_TOP + 1)); E4M3 ends at 1.75 * 2^8
-    static constexpr int Q_TOP = QK8 ? 7 : 14;
+    static constexpr uint32_t Q_BYTES = TERMS * 2 * NB * NQ * 32 * 8;  // [term][half][block][column tile][lane] 8 B
+    static constexpr int Q_TOP = 14;  // queries are scaled to a maximum in [2^14, 2^15): f16 keeps 2^-38 of it
     static constexpr uint32_t MERGE_BYTES = kWarps * MT * 32 * 16;
     static constexpr uint32_t SMEM = kWarps * R::STAGES * R::STAGE + Q_BYTES + MERGE_BYTES;
     static constexpr uint32_t MIN_CTAS = NQ * HD <= 256 ? 2 : 1;
@@ -417,53 +402,35 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
         }
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
-            if constexpr (TT::QK8) {
+            uint32_t a[2][4];
 #pragma unroll
-                for (uint32_t n = 0; n < NQ; ++n) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                    for (uint32_t z = 0; z < 2; ++z) {
+                for (uint32_t i = 0; i < 2; ++i) {
+                    if constexpr (FMT == FMT_FP8) {
+                        e4m3x4_to_f16(kw[i][h * CW + b], a[h][i], a[h][2 + i]);
+                    } else {
+                        uint32_t f[4];
+                        decode_word_f16(kw[i][h * CW + b / 2], f);
+                        a[h][i] = f[2 * (b & 1)], a[h][2 + i] = f[2 * (b & 1) + 1];
+                    }
+                }
+#pragma unroll
+            for (uint32_t n = 0; n < NQ; ++n) {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t z = 0; z < TERMS; ++z)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
                         uint32_t qf[2];
                         if constexpr (TT::QREG)
-                            qf[0] = T.q[z * NB + b].x, qf[1] = T.q[z * NB + b].y;
+                            qf[0] = T.q[h * NB + b].x, qf[1] = T.q[h * NB + b].y;
                         else
-                            lds_words<2>(qs + (((z * NB + b) * NQ + n) * 32 + lane) * 8, qf);
-                        mma_e4m3_16832(acc, kw[0][b], kw[1][b], kw[0][CW + b], kw[1][CW + b], qf[0], qf[1]);
+                            lds_words<2>(qs + ((((z * 2 + h) * NB + b) * NQ + n) * 32 + lane) * 8, qf);
+                        mma_f16_16816(acc, a[h], qf[0], qf[1], acc);
                     }
-                    s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
-                    s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
-                }
-            } else {
-                uint32_t a[2][4];
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i) {
-                        if constexpr (FMT == FMT_FP8) {
-                            e4m3x4_to_f16(kw[i][h * CW + b], a[h][i], a[h][2 + i]);
-                        } else {
-                            uint32_t f[4];
-                            decode_word_f16(kw[i][h * CW + b / 2], f);
-                            a[h][i] = f[2 * (b & 1)], a[h][2 + i] = f[2 * (b & 1) + 1];
-                        }
-                    }
-#pragma unroll
-                for (uint32_t n = 0; n < NQ; ++n) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (uint32_t z = 0; z < TERMS; ++z)
-#pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            uint32_t qf[2];
-                            if constexpr (TT::QREG)
-                                qf[0] = T.q[h * NB + b].x, qf[1] = T.q[h * NB + b].y;
-                            else
-                                lds_words<2>(qs + ((((z * 2 + h) * NB + b) * NQ + n) * 32 + lane) * 8, qf);
-                            mma_f16_16816(acc, a[h], qf[0], qf[1], acc);
-                        }
-                    s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
-                    s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
-                }
+                s[n][0] += acc[0] * ks[0][b], s[n][1] += acc[1] * ks[0][b];
+                s[n][2] += acc[2] * ks[1][b], s[n][3] += acc[3] * ks[1][b];
             }
         }
     }
@@ -639,10 +606,9 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             for (uint32_t b = 0; b < NB; ++b) x[b] = r < cur.rows ? (float)src[b * 32 + lane] : 0.0f, amax = fmaxf(amax, fabsf(x[b]));
             amax = warp_max(amax);
             const int e = amax > 0.0f ? max(-112, min(127, (int)(__float_as_uint(amax) >> 23) - 127)) : 0;
-            const int up_by = TT::Q_TOP - e + (TT::QK8 && (__float_as_uint(amax) & 0x7FFFFFu) <= 0x600000u);
-            const float up = pow2(up_by);
+            const float up = pow2(TT::Q_TOP - e);
             if (lane == 0) {
-                rowf[r] = p.scale * pow2(max(-up_by, -126));
+                rowf[r] = p.scale * pow2(max(e - TT::Q_TOP, -126));
                 limit[r] = prefix ? (int32_t)len
                                   : (int32_t)len - (int32_t)p.q_len + 1 + (int32_t)ra.step;
             }
@@ -652,15 +618,6 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
                 const uint32_t c = lane >> 2, i = lane & 3;
                 const uint32_t tt = R::PAIR ? c / 2 : c & 3, h = R::PAIR ? c & 1 : c >> 2;
                 float y = x[b] * up;
-                if constexpr (TT::QK8) {
-#pragma unroll
-                    for (uint32_t z = 0; z < 2; ++z) {
-                        const uint32_t code = e4m3x2(y, 0.0f) & 0xFF;
-                        const uint32_t back = e4m3x2_to_f16x2(code);
-                        y -= __low2float(*reinterpret_cast<const __half2 *>(&back));
-                        qbuf[(((z * NB + b) * NQ + r / 8) * 32 + (r % 8) * 4 + tt) * 8 + h * 4 + i] = (uint8_t)code;
-                    }
-                } else
 #pragma unroll
                 for (uint32_t z = 0; z < TT::TERMS; ++z) {
                     const __half hy = __float2half_rn(y);
