@@ -754,11 +754,14 @@ struct Big {
     static constexpr uint32_t Q_BYTES = QT * REG * 128 * 128, KV_BYTES = REG * TN * 128;
     static constexpr uint32_t SMEM = Q_BYTES + 4 * KV_BYTES + 1024;
     static constexpr uint32_t THREADS = 17 * 32, DEQ = 256;
-    // tensor memory columns: two S buffers (with their P), then O
-    static constexpr uint32_t S_COLS = F32 ? 160 : 128, O_COL = 2 * S_COLS, COLS = 512;
+    // tensor memory columns: two S buffers (P takes the place of S), then O, then the sum of earlier O
+    static constexpr uint32_t S_COLS = F32 ? 96 : 128, O_COL = 2 * S_COLS, SUM_COL = O_COL + HD, COLS = 512;
+    // f32: O is added to a sum of its own every FLUSH tiles.  The MMA's accumulator cuts off what it adds; over the
+    // 1100 additions of 6000 positions that cost 2e-6 of the result.
+    static constexpr uint32_t FLUSH = F32 ? 8 : 1u << 30;
     // first column of term z of P for positions 16 ks .. 16 ks + 15 (8 columns), from the buffer's start
     static __device__ __forceinline__ uint32_t p_col(uint32_t z, uint32_t ks) {
-        return F32 ? 64 + 32 * z + 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks & 1);
+        return F32 ? 32 * z + 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks & 1);
     }
 };
 
@@ -789,11 +792,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        FP4X_I8(v, 0), FP4X_I8(v, 8), FP4X_I8(v, 16), FP4X_I8(v, 24)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : FP4X_R8(v, 0), FP4X_R8(v, 8)
+        : "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -921,8 +925,9 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             const int32_t low = __reduce_min_sync(~0u, limit);
             const uint32_t stop = min(sg.c1 * kChunk, sg.len);
             float m = kNoMax, l = 0.0f;
-            bool first_tile = true, good = true;
-            for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile) {
+            bool good = true;
+            uint32_t done = 0;  // tiles of the segment so far
+            for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile, ++done) {
                 const uint32_t buf = tile & 1, ph = (tile >> 1) & 1, sb = tmem + lanes + buf * BG::S_COLS;
                 good = good && warp_wait(&sfull[buf], ph);
                 tc::fence_after_sync();
@@ -957,26 +962,35 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                     break;
                 }
                 mx = fmaxf(mx, other) * p.scale;
-                const bool grow = mx > m + kLag;
-                if (__any_sync(~0u, grow)) {
-                    const float mn = grow ? mx : m, f = ex2(m - mn);
-                    m = mn, l *= f;
-                    if (!first_tile) {
-                        const uint32_t pt = tile - 1;
-                        good = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
-                        tc::fence_after_sync();
+                const bool grow = mx > m + kLag, any = __any_sync(~0u, grow);
+                const bool flush = F32 && done && done % BG::FLUSH == 0, summed = F32 && done > BG::FLUSH;
+                const float mn = grow ? mx : m, f = any ? ex2(m - mn) : 1.0f;
+                m = mn, l *= f;
+                if ((any && done) || flush) {  // O rescaled, or moved to the sum
+                    const uint32_t pt = tile - 1;
+                    good = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
+                    tc::fence_after_sync();
 #pragma unroll 1
-                        for (uint32_t c = 0; c < HD / 64; ++c) {
-                            const uint32_t at = tmem + lanes + BG::O_COL + (half * (HD / 64) + c) * 32;
-                            uint32_t y[32];
-                            tmem_ld32(at, y);
+                    for (uint32_t c = 0; c < HD / 32; ++c) {
+                        const uint32_t at = tmem + lanes + half * (HD / 2) + c * 16;
+                        uint32_t y[16];
+                        tmem_ld16(at + BG::O_COL, y);
 #pragma unroll
-                            for (uint32_t i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-                            tmem_st32(at, y);
+                        for (uint32_t i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                        if (!flush) tmem_st16(at + BG::O_COL, y);
+                        if constexpr (F32) {
+                            if (summed) {
+                                uint32_t z[16];
+                                tmem_ld16(at + BG::SUM_COL, z);
+#pragma unroll
+                                for (uint32_t i = 0; i < 16; ++i)
+                                    y[i] = __float_as_uint(fmaf(__uint_as_float(z[i]), f,
+                                                                flush ? __uint_as_float(y[i]) : 0.0f));
+                            }
+                            if (summed || flush) tmem_st16(at + BG::SUM_COL, y);
                         }
                     }
                 }
-                first_tile = false;
 #pragma unroll
                 for (uint32_t cc = 0; cc < CH; ++cc) {
                     const uint32_t c = half * CH + (CH - 1 - cc);
@@ -1037,6 +1051,16 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             for (uint32_t c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
+                if (F32 && done > BG::FLUSH) {
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        uint32_t z[16];
+                        tmem_ld16(tmem + lanes + BG::SUM_COL + c * 32 + h * 16, z);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i)
+                            x[h * 16 + i] = __float_as_uint(__uint_as_float(x[h * 16 + i]) + __uint_as_float(z[i]));
+                    }
+                }
                 if (live) {
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 2) {
@@ -1217,7 +1241,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
                 __syncwarp();
                 if (pending && !(ok = issue_pv())) break;
-                pending = true, opens = pos == start;
+                pending = true, opens = pos == start || (F32 && (pos - start) / TN % BG::FLUSH == 0);
             }
         }
         if (ok && pending) ok = issue_pv();
