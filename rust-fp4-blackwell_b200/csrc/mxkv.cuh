@@ -10,8 +10,7 @@ namespace mxkv {
 enum : uint32_t { FMT_FP8 = FP4X_MXFP8, FMT_FP4 = FP4X_MXFP4 };
 
 // Device view of a cache.  Offsets into it are 64-bit (a pool of long contexts passes
-// 4 GB), those within a page 32-bit: one widening multiply-add makes an address, where
-// 64-bit strides took a fifth of the attention kernels' instructions.
+// 4 GB), those within a page 32-bit: one widening multiply-add makes an address.
 struct Cache {
     uint8_t *k, *ks, *v, *vs;
     uint32_t page_stride, scale_stride;  // bytes between pages

@@ -1263,7 +1263,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 // wrote whole has nothing to join.
 template <uint32_t HD, typename T>
 __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr uint32_t W = 4, V = HD / 32, U = 4, LIST = 512;  // a lane holds V dimensions
+    constexpr uint32_t W = 4, V = HD / 32, U = 4, LIST = 64;  // a lane holds V dimensions
     __shared__ float sm[W], sl[W], so[W][HD];
     __shared__ const float *ml_of[LIST], *o_of[LIST];
     const uint32_t row = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
