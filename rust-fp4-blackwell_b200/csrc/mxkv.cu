@@ -44,11 +44,8 @@ __device__ __forceinline__ uint32_t e8m0_of(float amax, int emax) {
     return (uint32_t)max(0, min(254, f - emax + 127));
 }
 
-// 2^(127 - e) as two factors, so that e = 254 and e = 0 stay exact.
-__device__ __forceinline__ void inv_scale(uint32_t e, float &a, float &b) {
-    const int h = 127 - (int)e, h0 = h / 2;
-    a = __uint_as_float((uint32_t)(h0 + 127) << 23), b = __uint_as_float((uint32_t)(h - h0 + 127) << 23);
-}
+// 2^(127 - e): e is at most 252 (amax below 2^128), so this is a normal number.
+__device__ __forceinline__ float inv_scale(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -56,18 +53,27 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// Two scaled values -> E2M1 codes: nearest level, ties to the smaller magnitude, -0 as
-// +0.  The conversion rounds ties to even; every tie has at most two mantissa bits, so
-// one unit less in the last place turns ties (and exact levels, harmlessly) downwards.
-__device__ __forceinline__ float below_tie(float v) {
-    const uint32_t u = __float_as_uint(v);
+// x times 2^(127 - e) for the E2M1 conversion, which rounds ties to even where the rule is
+// down, and with -0 as +0.  Every tie has at most two mantissa bits: one unit less in the
+// last place turns ties (and exact levels, harmlessly) downwards.  An f32 value one unit
+// above a tie must keep it, so the unit goes only where the low bits are zero; a bf16 value
+// has no such neighbour, and a factor of 1 - 2^-24 in the scale does it for all.
+template <typename T>
+__device__ __forceinline__ float scaled_e2m1(float x, float s);
+template <>
+__device__ __forceinline__ float scaled_e2m1<__nv_bfloat16>(float x, float s) {
+    return fmaf(x, s * 0.999999940395355224609375f, 0.0f);
+}
+template <>
+__device__ __forceinline__ float scaled_e2m1<float>(float x, float s) {
+    const uint32_t u = __float_as_uint(x * s);
     return __uint_as_float((u << 1) == 0 ? 0u : (u & 0x1FFFFFu) ? u : u - 1);
 }
 __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
     uint32_t r;
     asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
         : "=r"(r)
-        : "f"(below_tie(hi)), "f"(below_tie(lo)));
+        : "f"(hi), "f"(lo));
     return r;
 }
 
@@ -91,8 +97,9 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, flo
 // 2t and 2t + 1, dimensions 8t..8t+7 of every 32-block, so it moves 16-byte pieces on
 // both sides and a block's maximum takes two shuffles.  Bound by HBM: 131072 rows of
 // 8 x 128 MXFP8 to bf16 take 124 us (0.98 of the measured rate), 16384 bf16 rows to MXFP4
-// 26 us (85 MB; the chain load - maximum - store leaves 3.2 TB/s).  Shuffles that name four
-// lanes instead of the whole warp took 33 us.
+// 19.8 us (85 MB, 4.3 TB/s), f32 rows to MXFP8 30.7 us (5.5 TB/s).  For MXFP4 the ALU came
+// first: 33 us with shuffles that name four lanes instead of the whole warp, 26 us with the
+// f32 tie rule (below) for bf16 rows too.
 template <uint32_t HD>
 struct RowId {
     uint32_t t, head, is_v, token;
@@ -156,10 +163,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(Cache c, uint32_t n, con
         amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
         uint32_t e = e8m0_of(amax, FMT == FMT_FP8 ? 8 : 2);
-        float s0, s1;
-        inv_scale(e, s0, s1);
+        const float s = inv_scale(e);
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) x[b][j] = x[b][j] * s0 * s1;
+        for (uint32_t j = 0; j < 8; ++j) x[b][j] = FMT == FMT_FP8 ? x[b][j] * s : scaled_e2m1<T>(x[b][j], s);
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {  // chunk 2t + h: its four codes of block b at position 4 b
             const float *y = x[b] + 4 * h;

@@ -119,6 +119,27 @@ def test_append_special_values(fmt):
     assert torch.equal(k.isnan(), v.isnan())
 
 
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_append_bf16_ties_and_zeros(fmt):
+    """Every bf16 value between 2^-4 and 8 beside a fixed block maximum, both signs, zeros of both signs."""
+    bits = np.concatenate([np.arange(0x3D80, 0x4100), [0]]).astype(np.uint32)
+    vals = (bits << 16).view(np.float32)
+    vals = np.concatenate([vals, -vals])
+    n = -(-len(vals) // 62)
+    rows = np.zeros((n, 1, 64), np.float32)
+    body = np.zeros(n * 62, np.float32)
+    body[: len(vals)] = vals
+    rows[:, 0, :31], rows[:, 0, 32:63] = body.reshape(n, 62)[:, :31], body.reshape(n, 62)[:, 31:]
+    rows[:, 0, 31], rows[:, 0, 63] = 7.0, -7.5
+    cache = ops.MxKvCache.empty(-(-n // 16), 1, 64, 16, fmt)
+    x = torch.from_numpy(rows).to(torch.bfloat16).cuda()
+    assert torch.equal(x.float().cpu(), torch.from_numpy(rows))
+    ops.kv_append_mx(cache, torch.arange(n, dtype=torch.int32, device="cuda"), x, x)
+    c, s = R.encode(rows, fmt)
+    assert np.array_equal(cache.k[:, 0].flatten(0, 1)[:n].cpu().numpy(), c[:, 0])
+    assert np.array_equal(cache.v_scales[:, 0].flatten(0, 1)[:n].cpu().numpy(), s[:, 0])
+
+
 def test_slots_past_the_cache_are_skipped_and_reported():
     cache = ops.MxKvCache.empty(2, 2, 64, 16, "mxfp8")
     cache.k.fill_(1), cache.v.fill_(1), cache.k_scales.fill_(127), cache.v_scales.fill_(127)
