@@ -888,6 +888,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     __shared__ __align__(8) uint8_t no_page[4][8];
     __shared__ uint32_t tmem_base;
     __shared__ float halfmax[2][2][ROWS], halfsum[2][ROWS];
+    __shared__ uint32_t lost[4];  // a wait of either warp of these 32 rows ran out at a segment's end
     uint8_t *smem = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     uint8_t *qs = smem, *ks = smem + BG::Q_BYTES, *vs = ks + 2 * BG::KV_BYTES;
     const Job &job = prefix ? p.prefix : p.own;
@@ -899,6 +900,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             mbar_init(&pready[i], 8);
         }
         mbar_init(&done, 1);
+        lost[0] = lost[1] = lost[2] = lost[3] = 0;
         fence_mbar_init();
     }
     if (warp == 16) {
@@ -1037,8 +1039,10 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             good = good && warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
             tc::fence_after_sync();
             halfsum[half][row] = l;
+            if (!good && lane == 0) lost[quad] = 1;
             meet();
             l = halfsum[0][row] + halfsum[1][row];
+            ok = *(volatile uint32_t *)&lost[quad] == 0;  // both leave or neither
             const uint64_t out_row = (uint64_t)ra.token * p.n_heads + ra.head;
             const bool whole = sg.whole(), live = row < sg.rows;
             float *dst = nullptr;
@@ -1077,7 +1081,6 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
             }
             tc::fence_before_sync();
-            ok = good;
         }
     } else if (warp < 16) {
         // ================================================= codes -> bf16 images
