@@ -257,14 +257,31 @@ struct Ring {
     static constexpr bool PAIR = CHUNK < 16;  // both K chunks of a position in one load
     static constexpr uint32_t K_OFF = 0, V_OFF = 16 * B, KS_OFF = 32 * B, VS_OFF = KS_OFF + 16 * NB;
     static constexpr uint32_t STAGE = VS_OFF + 16 * NB;
-    // two CTAs per SM share 227 KB with their 16 or 32 KB merge buffers
-    static constexpr uint32_t STAGES = STAGE > 3000 ? 2 : STAGE > 2000 ? 3 : 4;
     static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t piece) {
         if (B == 128) return row * B + ((piece ^ (row & 6) ^ ((row & 1) << 2)) << 4);
         const uint32_t slot = row ^ ((row >> 2) & 1);
         return slot * B + ((B == 64 ? piece ^ (row & 2) : piece) << 4);
     }
 };
+
+__device__ __forceinline__ float lds1(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts1(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts4(uint32_t a, float4 v) {
+    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+// CTAs of attn_mx_kernel that share an SM, by its rows / 8 x dimensions: two while O and, for f32 queries, the sums of
+// it (Tile::SUMS) leave room for a second one.
+__host__ __device__ constexpr bool two_ctas(uint32_t nq_hd, bool f32) { return nq_hd < 256 || (nq_hd == 256 && !f32); }
 
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
 struct Tile {
@@ -273,14 +290,54 @@ struct Tile {
     static constexpr bool QREG = NQ == 1 && !F32;
     static constexpr uint32_t Q_BYTES = TERMS * 2 * NB * NQ * 32 * 8;  // [term][half][block][column tile][lane] 8 B
     static constexpr int Q_TOP = 14;  // queries are scaled to a maximum in [2^14, 2^15): f16 keeps 2^-38 of it
-    static constexpr uint32_t MERGE_BYTES = kWarps * MT * 32 * 16;
-    static constexpr uint32_t SMEM = kWarps * R::STAGES * R::STAGE + Q_BYTES + MERGE_BYTES;
-    static constexpr uint32_t MIN_CTAS = NQ * HD <= 256 ? 2 : 1;
+    static constexpr uint32_t MERGE_BYTES = kWarps * MT * 32 * 16;  // O of one column tile, all warps
+    static constexpr uint32_t MIN_CTAS = two_ctas(NQ * HD, F32) ? 2 : 1;
+    // The MMA's accumulator cuts off what it adds (up to an ulp, always towards zero): over the 768 dependent
+    // additions of 32768 positions that took 6.0e-6 of an f32 result, over 131072 positions 3.1e-5.  So every PERIOD
+    // tiles (48 additions, 32 for bf16 queries) O moves to an f32 sum that each lane keeps in shared memory, where the
+    // warps' results meet later: 5.9e-7 at any length.  It costs 1.5 % at 8 rows x 128 (64 sequences of up to 16384,
+    // MXFP8, bf16: 219 -> 222 us) and 11 % where f32 queries give up the second CTA for it (16 rows x 128, 64 of up to
+    // 8192: 214 -> 238 us; sums after every tile instead, in registers: 287 us).  bf16 queries with 256 row-dimensions
+    // keep the second CTA (184 us; 204 with one) and the chain: 2 additions a tile, up to 1e-4 of a result over 131072
+    // positions in one CTA, where bf16 has steps of 4e-3 to 8e-3 of it.
+    static constexpr bool SUMS = !(MIN_CTAS == 2 && NQ * HD == 256);
+    static constexpr uint32_t PERIOD = 16, SUM_BYTES = (SUMS ? NQ : 1) * MERGE_BYTES;
+    static constexpr uint32_t STAGES = MIN_CTAS == 1 && NQ * HD == 256 ? 4 : R::STAGE > 3000 ? 2 : R::STAGE > 2000 ? 3 : 4;
+    static constexpr uint32_t SMEM = kWarps * STAGES * R::STAGE + Q_BYTES + SUM_BYTES;
+    static_assert((SMEM + 5120) * MIN_CTAS <= 228 * 1024, "the CTAs of an SM share its memory (5 KB: static and reserved)");
 
     float o[MT][NQ][4];
     float m[NQ][2], l[NQ][2];
     uint2 q[QREG ? 2 * NB : 1];
 
+    // This lane's part of a sum, by column tile and 16-row tile of O.
+    static __device__ __forceinline__ uint32_t sum_at(uint32_t qs, uint32_t n, uint32_t i) {
+        return qs + Q_BYTES + (((n * kWarps + threadIdx.x / 32) * MT + i) * 32 + threadIdx.x % 32) * 16;
+    }
+    __device__ __forceinline__ void to_sum(uint32_t qs, bool add) {
+#pragma unroll
+        for (uint32_t n = 0; n < NQ; ++n)
+#pragma unroll
+            for (uint32_t i = 0; i < MT; ++i) {
+                const uint32_t at = sum_at(qs, n, i);
+                float4 y = make_float4(o[i][n][0], o[i][n][1], o[i][n][2], o[i][n][3]);
+                if (add) {
+                    const float4 z = lds4(at);
+                    y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                }
+                sts4(at, y);
+                o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+            }
+    }
+    __device__ __forceinline__ void from_sum(uint32_t qs) {
+#pragma unroll
+        for (uint32_t n = 0; n < NQ; ++n)
+#pragma unroll
+            for (uint32_t i = 0; i < MT; ++i) {
+                const float4 z = lds4(sum_at(qs, n, i));
+                o[i][n][0] += z.x, o[i][n][1] += z.y, o[i][n][2] += z.z, o[i][n][3] += z.w;
+            }
+    }
     __device__ __forceinline__ void reset() {
 #pragma unroll
         for (uint32_t i = 0; i < MT; ++i)
@@ -359,8 +416,8 @@ __device__ __forceinline__ void value_fragments(const uint32_t (&vw)[4][Ring<FMT
 // One tile from the ring into the running softmax.  `left` positions of the tile
 // exist (0: a page outside the cache); lim[8 n + j] is the limit of column 2 t + j of tile n.
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, bool F32>
-__device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ring, uint32_t qs, uint32_t left,
-                                          bool masked, const int32_t *lim, int32_t first, const float *rf,
+__device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ring, uint32_t qs, bool summed,
+                                          uint32_t left, bool masked, const int32_t *lim, int32_t first, const float *rf,
                                           uint32_t lane) {
     using R = Ring<FMT, HD>;
     using TT = Tile<FMT, HD, NQ, F32>;
@@ -464,6 +521,13 @@ __device__ __forceinline__ void take_tile(Tile<FMT, HD, NQ, F32> &T, uint32_t ri
                 T.l[n][j] *= f;
 #pragma unroll
                 for (uint32_t i = 0; i < TT::MT; ++i) T.o[i][n][j] *= f, T.o[i][n][2 + j] *= f;
+                if (TT::SUMS && summed) {
+#pragma unroll 1
+                    for (uint32_t i = 0; i < TT::MT; ++i) {
+                        const uint32_t at = TT::sum_at(qs, n, i) + 4 * j;
+                        sts1(at, lds1(at) * f), sts1(at + 8, lds1(at + 8) * f);
+                    }
+                }
             }
     }
     uint32_t p[TT::PTERMS][NQ][2];
@@ -549,8 +613,8 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
     __shared__ int32_t limit[ROWS];
     const Job &job = prefix ? p.prefix : p.own;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * R::STAGES * R::STAGE;
-    uint8_t *qbuf = smem + kWarps * R::STAGES * R::STAGE;
+    const uint32_t ring = smem_u32(smem) + warp * TT::STAGES * R::STAGE;
+    uint8_t *qbuf = smem + kWarps * TT::STAGES * R::STAGE;
     float4 *merge = reinterpret_cast<float4 *>(qbuf + TT::Q_BYTES);
     const Located loc = locate<kWarps * 32>(job, p.c.n_kv * job.row_tiles, scan, where);
     // The walk over the segments lives in shared memory, one copy per warp: its state
@@ -570,10 +634,10 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             if ((j & 31) == 0) ids = j + lane < n_tiles ? table[((c0 + j + lane) * kWarps + warp) * 16 >> p.c.page_shift] : 0;
             const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
             const int32_t page = __shfl_sync(~0u, ids, j & 31);
-            issue_tile<FMT, HD>(p.c, ring + j % R::STAGES * R::STAGE, page, head,
+            issue_tile<FMT, HD>(p.c, ring + j % TT::STAGES * R::STAGE, page, head,
                                 first & ((1u << p.c.page_shift) - 1), min(16u, len - first), lane);
             const bool out = (uint32_t)page >= p.c.n_pages;
-            bad = (bad & ~(1u << j % R::STAGES)) | ((uint32_t)out << j % R::STAGES);
+            bad = (bad & ~(1u << j % TT::STAGES)) | ((uint32_t)out << j % TT::STAGES);
             if (out && lane == 0) raise_device_error(DEVERR_BAD_ARG);
         }
         cp_async_commit();
@@ -592,7 +656,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         n_tiles = sg.c1 - c0;
         while (n_tiles && (c0 + n_tiles - 1) * kWarps + warp >= tiles) --n_tiles;
 #pragma unroll
-        for (uint32_t j = 0; j < R::STAGES; ++j) issue(j);
+        for (uint32_t j = 0; j < TT::STAGES; ++j) issue(j);
         return true;
     };
     uint32_t slot_of = 0;
@@ -648,19 +712,25 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
             for (uint32_t i = 0; i < 2 * NB; ++i) tile.q[i] = reinterpret_cast<const uint2 *>(qbuf)[i * 32 + lane];
         }
         uint32_t stage = 0;
-        for (uint32_t j = 0; j < n_tiles; ++j) {
-            const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
-            cp_async_wait<R::STAGES - 1>();
-            __syncwarp();  // every lane's copies of the tile have landed
-            uint32_t left = min(16u, len - first);
-            bool masked = (int32_t)(first + 16) > lowest || left < 16;
-            if ((bad >> stage) & 1) left = 0, masked = true;
-            take_tile<FMT, HD, NQ, F32>(tile, ring + stage * R::STAGE, smem_u32(qbuf), left, masked, limit + 2 * t,
-                                        (int32_t)first, rf, lane);
-            stage = stage + 1 == R::STAGES ? 0 : stage + 1;
-            __syncwarp();  // every lane has read the stage
-            issue(j + R::STAGES);
+        bool summed = false;
+        for (uint32_t j = 0; j < n_tiles;) {
+            const uint32_t to = TT::SUMS ? min(n_tiles, j + TT::PERIOD) : n_tiles;
+            for (; j < to; ++j) {
+                const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
+                cp_async_wait<TT::STAGES - 1>();
+                __syncwarp();  // every lane's copies of the tile have landed
+                uint32_t left = min(16u, len - first);
+                bool masked = (int32_t)(first + 16) > lowest || left < 16;
+                if ((bad >> stage) & 1) left = 0, masked = true;
+                take_tile<FMT, HD, NQ, F32>(tile, ring + stage * R::STAGE, smem_u32(qbuf), summed, left, masked, limit + 2 * t,
+                                            (int32_t)first, rf, lane);
+                stage = stage + 1 == TT::STAGES ? 0 : stage + 1;
+                __syncwarp();  // every lane has read the stage
+                issue(j + TT::STAGES);
+            }
+            if (TT::SUMS && j < n_tiles) tile.to_sum(smem_u32(qbuf), summed), summed = true;
         }
+        if (summed) tile.from_sum(smem_u32(qbuf));
         more = open(slot_of);  // its first copies run under the joining of this one
         // ---- join the warps
 #pragma unroll
@@ -1375,18 +1445,19 @@ struct Plan {
     uint32_t own_ctas, prefix_ctas;
     uint64_t own_slots, prefix_slots, row_slots, starts;  // floats
 };
-// CTAs of a job that run at once per SM: see Tile::MIN_CTAS.
-inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows) { return tile_rows * hd <= 2048 ? 2 : 1; }
+// CTAs of a job that run at once per SM.
+inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows, bool f32) { return two_ctas(tile_rows / 8 * hd, f32) ? 2 : 1; }
 
+// The plan for bf16 queries needs at least the workspace of that for f32 (it has at least the CTAs).
 Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uint32_t q_len, uint32_t prefix_len,
-               uint32_t max_len) {
+               uint32_t max_len, bool f32) {
     Plan pl = {};
     const uint64_t rows = (uint64_t)(n_heads / n_kv) * q_len, all = rows * batch;
     const uint32_t sms = (uint32_t)num_sms();
     auto job = [&](uint32_t seqs, uint32_t len, uint64_t r, uint32_t &tile_rows, uint32_t &ctas, uint64_t &slots) {
         tile_rows = tile_rows_of(r);
         const uint64_t chunks = ((uint64_t)len + kChunk - 1) / kChunk * seqs * n_kv * ((r + tile_rows - 1) / tile_rows);
-        const uint64_t room = (uint64_t)sms * ctas_per_sm(hd, tile_rows);
+        const uint64_t room = (uint64_t)sms * ctas_per_sm(hd, tile_rows, f32);
         ctas = (uint32_t)(chunks < room ? chunks : room);  // more would idle
         slots = 2ull * ctas * tile_rows * (hd + 2);
     };
@@ -1417,7 +1488,6 @@ int launch_with_smem(const char *who, cudaStream_t st, K kernel, bool (&ready)[6
 template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
 int launch_stream(const char *who, cudaStream_t st, const AttnParams &p, bool prefix) {
     using TT = Tile<FMT, HD, NQ, sizeof(T) == 4>;
-    static_assert(TT::MIN_CTAS == (8 * NQ * HD <= 2048 ? 2 : 1), "ctas_per_sm and the launch bounds agree");
     static bool ready[64] = {};
     return launch_with_smem(who, st, attn_mx_kernel<FMT, HD, NQ, T>, ready, (prefix ? p.prefix : p.own).ctas,
                             kWarps * 32, TT::SMEM, p, prefix);
@@ -1471,7 +1541,7 @@ int launch_attn(const char *who, cudaStream_t st, const fp4x_mxkv *cache, uint32
     FP4X_REQUIRE(aligned(q, 16) && aligned(out, 16) && q_stride % (dtype == FP4X_F32 ? 4 : 8) == 0,
                  "%s: rows of q and out must be 16-byte aligned", who);
     FP4X_REQUIRE(q_stride >= (uint64_t)n_heads * hd, "%s: q_stride below n_heads * head_dim", who);
-    const Plan pl = make_plan(p.c.n_kv, hd, batch, n_heads, q_len, prefix_len, max_len);
+    const Plan pl = make_plan(p.c.n_kv, hd, batch, n_heads, q_len, prefix_len, max_len, dtype == FP4X_F32);
     const size_t need = (pl.starts + pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float);
     FP4X_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
                  "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need, workspace_bytes);
@@ -1505,7 +1575,7 @@ extern "C" size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t 
                                                uint32_t q_len, uint32_t prefix_len, uint32_t max_len) {
     if (!cache || !cache->n_kv_heads || n_heads < cache->n_kv_heads) return 0;
     const mxkv::Plan pl =
-        mxkv::make_plan(cache->n_kv_heads, cache->head_dim, batch, n_heads, q_len, prefix_len, max_len);
+        mxkv::make_plan(cache->n_kv_heads, cache->head_dim, batch, n_heads, q_len, prefix_len, max_len, false);
     return (size_t)((pl.starts + pl.own_slots + pl.prefix_slots + pl.row_slots * 2) * sizeof(float));
 }
 
