@@ -830,9 +830,10 @@ struct Big {
     static constexpr uint32_t THREADS = 17 * 32, DEQ = 256;
     // tensor memory columns: two S buffers (P takes the place of S), then O, then the sum of earlier O
     static constexpr uint32_t S_COLS = F32 ? 96 : 128, O_COL = 2 * S_COLS, SUM_COL = O_COL + HD, COLS = 512;
-    // f32: O is added to a sum of its own every FLUSH tiles.  The MMA's accumulator cuts off what it adds; over the
-    // 1100 additions of 6000 positions that cost 2e-6 of the result.
-    static constexpr uint32_t FLUSH = F32 ? 8 : 1u << 30;
+    // O is added to a sum of its own every FLUSH tiles, because the MMA's accumulator cuts off what it adds (see
+    // Tile::SUMS).  f32: 24 additions a time, 4.3e-7 of sums of one sign (every 8 tiles: 5.0e-6; every tile: 4.0e-7
+    // for up to 3 % of the time).  bf16: 128, a few 1e-6 (never: 1.5 % faster on 32768 positions).
+    static constexpr uint32_t FLUSH = F32 ? 2 : 8;
     // first column of term z of P for positions 16 ks .. 16 ks + 15 (8 columns), from the buffer's start
     static __device__ __forceinline__ uint32_t p_col(uint32_t z, uint32_t ks) {
         return F32 ? 32 * z + 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks & 1);
@@ -1039,7 +1040,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
                 mx = fmaxf(mx, other) * p.scale;
                 const bool grow = mx > m + kLag, any = __any_sync(~0u, grow);
-                const bool flush = F32 && done && done % BG::FLUSH == 0, summed = F32 && done > BG::FLUSH;
+                const bool flush = done && done % BG::FLUSH == 0, summed = done > BG::FLUSH;
                 const float mn = grow ? mx : m, f = any ? ex2(m - mn) : 1.0f;
                 m = mn, l *= f;
                 if ((any && done) || flush) {  // O rescaled, or moved to the sum
@@ -1054,17 +1055,14 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
                         if (!flush) tmem_st16(at + BG::O_COL, y);
-                        if constexpr (F32) {
-                            if (summed) {
-                                uint32_t z[16];
-                                tmem_ld16(at + BG::SUM_COL, z);
+                        if (summed) {
+                            uint32_t z[16];
+                            tmem_ld16(at + BG::SUM_COL, z);
 #pragma unroll
-                                for (uint32_t i = 0; i < 16; ++i)
-                                    y[i] = __float_as_uint(fmaf(__uint_as_float(z[i]), f,
-                                                                flush ? __uint_as_float(y[i]) : 0.0f));
-                            }
-                            if (summed || flush) tmem_st16(at + BG::SUM_COL, y);
+                            for (uint32_t i = 0; i < 16; ++i)
+                                y[i] = __float_as_uint(fmaf(__uint_as_float(z[i]), f, flush ? __uint_as_float(y[i]) : 0.0f));
                         }
+                        if (summed || flush) tmem_st16(at + BG::SUM_COL, y);
                     }
                 }
 #pragma unroll
@@ -1087,12 +1085,10 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) {
                             const float2 e = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
-                            if (z + 1 == BG::PT) {
-                                y[i] = pack_bf16x2(e.x, e.y);
-                            } else {  // the term cut off, not rounded: its upper half is the term
-                                y[i] = __byte_perm(x[2 * i], x[2 * i + 1], 0x7632);
-                                const float2 r = add2(e, make_float2(-__uint_as_float(x[2 * i] & 0xFFFF0000u),
-                                                                     -__uint_as_float(x[2 * i + 1] & 0xFFFF0000u)));
+                            y[i] = pack_bf16x2(e.x, e.y);
+                            if (z + 1 < BG::PT) {
+                                const float2 r = add2(e, make_float2(__uint_as_float((y[i] << 16) ^ 0x80000000u),
+                                                                     __uint_as_float((y[i] & 0xFFFF0000u) ^ 0x80000000u)));
                                 x[2 * i] = __float_as_uint(r.x), x[2 * i + 1] = __float_as_uint(r.y);
                             }
                         }
@@ -1129,7 +1125,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             for (uint32_t c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
-                if (F32 && done > BG::FLUSH) {
+                if (done > BG::FLUSH) {
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
                         uint32_t z[16];
@@ -1318,7 +1314,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
                 __syncwarp();
                 if (pending && !(ok = issue_pv())) break;
-                pending = true, opens = pos == start || (F32 && (pos - start) / TN % BG::FLUSH == 0);
+                pending = true, opens = (pos - start) / TN % BG::FLUSH == 0;
             }
         }
         if (ok && pending) ok = issue_pv();

@@ -55,7 +55,8 @@ def _close(got, want, mass, size, n):
 
 
 @pytest.mark.parametrize("group,hd,fmt", [(4, 128, "mxfp8"), (8, 64, "mxfp4"), (16, 64, "mxfp8"), (16, 128, "mxfp8"),
-                                          (9, 128, "mxfp4"), (32, 64, "mxfp4"), (17, 128, "mxfp8")])
+                                          (9, 128, "mxfp4"), (32, 64, "mxfp4"), (17, 128, "mxfp8"),
+                                          (64, 128, "mxfp8"), (40, 64, "mxfp4")])
 def test_sums_do_not_drift_with_the_length(group, hd, fmt):
     """Near-equal scores and values of one sign over 32768 positions, a segment per CTA: the f32 sums stay f32 sums."""
     n, n_kv, batch, page = 32768, 8, 37, 64
@@ -76,7 +77,7 @@ def test_sums_do_not_drift_with_the_length(group, hd, fmt):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("group,hd,fmt", [(1, 128, "mxfp8"), (7, 64, "mxfp4"), (12, 128, "mxfp8"), (16, 64, "mxfp4"),
-                                          (32, 64, "mxfp8"), (20, 128, "mxfp4")])
+                                          (32, 64, "mxfp8"), (20, 128, "mxfp4"), (33, 128, "mxfp8"), (64, 64, "mxfp4")])
 def test_maximum_that_grows_late(group, hd, fmt, dtype):
     """Single positions whose scores pass all before by more than the kernels leave standing (16 powers of two), with as
     much of the probability as the thousands before them: what was summed before is rescaled, in registers and out."""
@@ -97,3 +98,24 @@ def test_maximum_that_grows_late(group, hd, fmt, dtype):
         got = ops.attn_paged_mx(cache, q, table, lens)
         seen = (torch.arange(n, device="cuda") < length).expand(batch, n)
         _close(got[:, 0], *_definition(q[:, 0], k, v, seen), n)
+
+
+@pytest.mark.parametrize("group,hd,fmt", [(4, 128, "mxfp8"), (64, 128, "mxfp8"), (48, 64, "mxfp4")])
+def test_bf16_results_have_no_bias(group, hd, fmt):
+    """bf16 results over 32768 positions, spread over a power of two: their rounding errors average out, a sum that
+    loses a little with every addition does not."""
+    n, n_kv, batch, page = 32768, 8, 37, 64
+    g = _gen(group)
+    spread = torch.exp2(torch.arange(hd, device="cuda") / hd)
+    cache, k, v = _cache(torch.randn((n, n_kv, hd), generator=g, device="cuda"),
+                         torch.randn((n, n_kv, hd), generator=g, device="cuda").abs() * spread, page, fmt)
+    q = (torch.randn((batch, 1, n_kv * group, hd), generator=g, device="cuda") * 0.5).bfloat16()
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    got = ops.attn_paged_mx(cache, q, table, lens)[:, 0]
+    want, mass, size = _definition(q[:, 0], k, v, torch.ones((batch, n), dtype=torch.bool, device="cuda"))
+    _close(got, want, mass, size, n)
+    # at most 128 additions that cut off up to an ulp of an evenly growing sum (64 x 2^-23); rounding errors of at most
+    # 2^-8 of the result, evenly spread (deviation 2^-8 / sqrt(3)): five deviations of their mean
+    bias = float(((got.double() - want) / want).mean())
+    assert abs(bias) <= 2.0 ** -17 + 5 * 2.0 ** -8 / (3 * want.numel()) ** 0.5, bias
