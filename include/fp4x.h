@@ -307,7 +307,8 @@ FP4X_API int llama_attn_shared_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, 
  * q_i = 1 at d_i); draft_lens[b] <= k drafts count (NULL: k); temperature NULL: 1.
  * A temperature that is not above 1e-30 (0, negative, NaN) decodes greedily: a draft
  * is accepted if it is the argmax (ties to the lowest index), the last token is the
- * argmax, uniforms and noise are not used.  NaN logits count as -inf.  A residual or
+ * argmax, uniforms and noise are not used.  A temperature of +inf makes all
+ * tokens with a logit above -inf equally likely.  NaN logits count as -inf.  A residual or
  * distribution without any mass falls back to p, then to the argmax.  A draft id
  * outside the vocabulary is rejected.  Outputs: accepted[b]; tokens [batch][k + 1] =
  * the accepted drafts, the sampled token, then -1; logprobs (NULL: not wanted) =

@@ -88,11 +88,12 @@ struct Raw {
 __device__ __forceinline__ uint32_t drafts_of(const Params &p, uint32_t b) {
     return p.lens ? (uint32_t)min(max(p.lens[b], 0), (int32_t)p.k) : p.k;
 }
-// log2(e) / T, or log2(e) for greedy sequences (their log-probabilities are at T = 1).
+// log2(e) / T, or log2(e) for greedy sequences (their log-probabilities are at T = 1).  Never 0: a temperature of +inf
+// takes the smallest positive factor, with which a masked logit stays -inf (0 would make it NaN) and the others are alike.
 __device__ __forceinline__ float factor_of(const Params &p, uint32_t b, bool &greedy) {
     const float t = p.temp ? p.temp[b] : 1.0f;
     greedy = !(t > 1e-30f);
-    return greedy ? kLog2e : kLog2e / t;
+    return greedy ? kLog2e : fmaxf(kLog2e / t, 1.401298464324817e-45f);
 }
 
 __device__ __forceinline__ Stat join(const Stat &a, const Stat &b, float c) {

@@ -139,3 +139,19 @@ def test_verify_samples_the_target():
     p = torch.softmax(row.double(), -1).cpu().numpy()
     got = np.bincount(tok[:, 0].cpu().numpy(), minlength=V) / B
     assert np.all(np.abs(got - p) <= 5 * np.sqrt(p * (1 - p) / B))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("temp", [float("inf"), 3e38, 1e20])
+def test_verify_at_temperatures_without_end(temp, probs, dtype):
+    """+inf and very large temperatures: every token that is not masked is as likely as any other."""
+    for B, k, V in ((1, 1, 4), (6, 3, 1001), (3, 4, 9000)):
+        args = _case(B + V, B, k, V, dtype, probs)
+        args[0][0, :, V // 2:] = -torch.inf
+        args[0][-1, 0, 1] = torch.nan
+        t = torch.full((B,), temp, device="cuda")
+        t[1:B - 1:2] = 0.8  # beside ordinary ones
+        want = _check(args, temperature=t)
+        _check(args, temperature=t, draft_lens=torch.zeros(B, dtype=torch.int32, device="cuda"))
+        assert np.isfinite(want[2]).all()
