@@ -273,8 +273,8 @@ FP4X_API size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t ba
  * rows q_stride elements apart, 16-byte aligned), out the same shape, contiguous and
  * 16-byte aligned.  Sequence b holds lens[b] positions (device array; clamped to
  * 0..max_len), the q_len query tokens of this step included as the last ones: query
- * i attends to positions 0 .. lens[b] - q_len + i.  A query that sees no position
- * gives zeros.  page_table [batch] rows of table_stride page ids, at least
+ * i attends to positions 0 .. lens[b] - q_len + i; what the others hold (NaN
+ * included) has no influence on it.  A query that sees no position gives zeros.  page_table [batch] rows of table_stride page ids, at least
  * ceil(max_len / page_size) each; ids outside the cache are not read: their
  * positions are masked and the device error word is set.  Softmax scale
  * 1/sqrt(head_dim), statistics and sums in f32; the probabilities enter the tensor

@@ -1330,17 +1330,86 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     end_kernel(p, prefix);
 }
 
+// ---------------------------------------------------------------- hidden positions that are not finite
+// Of the last q_len positions of a sequence some queries see only the first ones.  The kernels above give the others the
+// probability 0, and 0 times a NaN (or a value past 2^128) in V is NaN.  That is rare, so they do not look: the join
+// does where a result is NaN, and if such a position holds one, it computes the row anew from what the row sees, with
+// plain f32 arithmetic (a CTA for one row, 128 positions at a time).
+
+// Dimension d of a cached row.
+template <uint32_t FMT, uint32_t HD>
+__device__ __forceinline__ float value_at(const uint8_t *codes, const uint8_t *scales, uint32_t d) {
+    const uint32_t at = (d % 32 / 4 * (HD / 32) + d / 32) * 4 + d % 4;
+    const uint32_t h = FMT == FMT_FP8 ? e4m3x2_to_f16x2(codes[at]) : e2m1x2_to_f16x2(codes[at / 2] >> (at % 2 * 4) & 15);
+    return __half2float(__ushort_as_half((unsigned short)h)) * e8m0_to_f32(scales[d / 32]);
+}
+
+// The page of position t of a row that sees the prefix and then `own` positions.
+__device__ __forceinline__ uint32_t page_of(const AttnParams &p, uint32_t seq, uint32_t t, uint32_t &row) {
+    const uint32_t before = p.prefix.ctas ? p.prefix.max_len : 0, u = t < before ? t : t - before;
+    row = u & ((1u << p.c.page_shift) - 1);
+    return t < before ? p.prefix.pages[u >> p.c.page_shift]
+                      : p.own.pages[(uint64_t)seq * p.own.table_stride + (u >> p.c.page_shift)];
+}
+
+template <uint32_t FMT, uint32_t HD, typename T>
+__device__ __noinline__ void redo_row(const AttnParams &p, uint32_t token, uint32_t head) {
+    __shared__ float qf[HD], prob[128], red[4];
+    const uint32_t seq = token / p.q_len, kvh = head / p.group, tid = threadIdx.x;
+    const uint32_t before = p.prefix.ctas ? p.prefix.max_len : 0, len = seq_len(p.own, seq);
+    const uint32_t seen = (uint32_t)max((int32_t)len - (int32_t)p.q_len + 1 + (int32_t)(token % p.q_len), 0), n = before + seen;
+    uint32_t row;
+    bool bad = false;
+    for (uint32_t i = tid; i < (len - seen) * HD; i += 128) {
+        const uint32_t page = page_of(p, seq, n + i / HD, row);
+        if (page >= p.c.n_pages) continue;
+        const float v = value_at<FMT, HD>(p.c.v + code_off<FMT, HD>(p.c, page, kvh, row),
+                                          p.c.vs + scale_off<HD>(p.c, page, kvh, row), i % HD);
+        bad |= !(fabsf(v) <= 3.40282347e+38f);
+    }
+    if (!__syncthreads_or(bad)) return;  // the NaN is the row's own
+    if (tid < HD) qf[tid] = (float)((const T *)p.q)[token * p.q_stride + head * HD + tid] * p.scale;
+    float m = kNoMax, l = 0.0f, o = 0.0f;
+    for (uint32_t t0 = 0; t0 < n; t0 += 128) {
+        __syncthreads();
+        float s = -INFINITY;
+        uint32_t page = t0 + tid < n ? page_of(p, seq, t0 + tid, row) : ~0u;
+        if (page < p.c.n_pages) {
+            const uint8_t *codes = p.c.k + code_off<FMT, HD>(p.c, page, kvh, row), *scales = p.c.ks + scale_off<HD>(p.c, page, kvh, row);
+            s = 0.0f;
+            for (uint32_t d = 0; d < HD; ++d) s = fmaf(qf[d], value_at<FMT, HD>(codes, scales, d), s);
+        }
+        const float mw = warp_max(s);
+        if (tid % 32 == 0) red[tid / 32] = mw;
+        __syncthreads();
+        const float mx = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), f = exp2f(m - mx);
+        prob[tid] = exp2f(s - mx);
+        __syncthreads();
+        m = mx, l *= f, o *= f;
+        for (uint32_t i = 0; i < min(128u, n - t0); ++i) {
+            l += prob[i];
+            page = page_of(p, seq, t0 + i, row);
+            if (page < p.c.n_pages && tid < HD)
+                o += prob[i] * value_at<FMT, HD>(p.c.v + code_off<FMT, HD>(p.c, page, kvh, row),
+                                                 p.c.vs + scale_off<HD>(p.c, page, kvh, row), tid);
+        }
+    }
+    if (tid < HD) ((T *)p.out)[((uint64_t)token * p.n_heads + head) * HD + tid] = (T)(l == 0.0f ? 0.0f : o / l);
+}
+
 // Joins the partial results of one output row: those of the CTAs that shared its
 // segment, and with a prefix those of both jobs.  The places of all partials are worked
 // out first, so that four warps can have four loads each in flight; a row that one CTA
 // wrote whole has nothing to join.
-template <uint32_t HD, typename T>
+template <uint32_t FMT, uint32_t HD, typename T>
 __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant__ AttnParams p) {
     constexpr uint32_t W = 4, V = HD / 32, U = 4, LIST = 64;  // a lane holds V dimensions
     __shared__ float sm[W], sl[W], so[W][HD];
     __shared__ const float *ml_of[LIST], *o_of[LIST];
     const uint32_t row = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t token = row / p.n_heads, head = row % p.n_heads, kvh = head / p.group;
+    const bool hides = p.q_len > 1 && p.own.ctas;  // some positions from some queries
+    T *out = (T *)p.out + (uint64_t)row * HD + threadIdx.x;
     pdl_wait();
     // partials of each job: the row's slot, or its place in the slots of CTAs first..last
     uint32_t n = 0, from[2], count[2], in_tile[2];
@@ -1360,7 +1429,13 @@ __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant
                             (uint64_t)(r / job.tile_rows * p.c.n_kv + kvh) * (chunks + kOpen) + kOpen;
         from[which] = cta_of(at, total[which], job.ctas);
         count[which] = cta_of(at + chunks - 1, total[which], job.ctas) - from[which] + 1;
-        if (count[which] == 1 && !job.row_slots) return;  // written whole (without a prefix)
+        if (count[which] == 1 && !job.row_slots) {  // written whole (without a prefix)
+            if (hides) {
+                const float y = threadIdx.x < HD ? (float)*out : 0.0f;
+                if (__syncthreads_or(y != y)) redo_row<FMT, HD, T>(p, token, head);
+            }
+            return;
+        }
         n += count[which];
     }
     float m = kNoMax, l = 0.0f, o[V];
@@ -1417,16 +1492,17 @@ __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant
 #pragma unroll
     for (uint32_t i = 0; i < V; ++i) so[warp][lane * V + i] = o[i];
     __syncthreads();
-    if (threadIdx.x >= HD) return;
     float mx = kNoMax, sum = 0.0f, acc = 0.0f;
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) mx = fmaxf(mx, sm[w]);
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) {
         const float f = exp2f(sm[w] - mx);
-        sum += sl[w] * f, acc += so[w][threadIdx.x] * f;
+        sum += sl[w] * f, acc += so[w][threadIdx.x % HD] * f;
     }
-    ((T *)p.out)[(uint64_t)row * HD + threadIdx.x] = (T)(sum == 0.0f ? 0.0f : acc / sum);
+    const float y = sum == 0.0f ? 0.0f : acc / sum;
+    if (threadIdx.x < HD) *out = (T)y;
+    if (hides && __syncthreads_or(y != y)) redo_row<FMT, HD, T>(p, token, head);
 }
 
 // ---------------------------------------------------------------- host
@@ -1508,7 +1584,7 @@ int launch_all(const char *who, cudaStream_t st, const AttnParams &p, uint64_t r
                                    : launch_tile<FMT, HD, T>(who, st, p, prefix);
     }
     if (rc != FP4X_OK) return rc;
-    const cudaError_t e = launch_pdl(attn_mx_join_kernel<HD, T>, dim3((uint32_t)rows), dim3(128), 0, st, p);
+    const cudaError_t e = launch_pdl(attn_mx_join_kernel<FMT, HD, T>, dim3((uint32_t)rows), dim3(128), 0, st, p);
     if (e != cudaSuccess) return set_error("%s: %s", who, cudaGetErrorString(e)), FP4X_ECUDA;
     return check_launch(who);
 }
