@@ -23,7 +23,8 @@ class Llama:
     """Random-weight Llama whose attention state lives in MxKvCache pages, one cache per layer."""
 
     def __init__(self, layers=2, dim=256, ffn=512, heads=8, kv_heads=2, head_dim=64, vocab=512, seed=1, max_pos=4096):
-        self.heads, self.kv_heads, self.hd, self.vocab = heads, kv_heads, head_dim, vocab
+        self.heads, self.kv_heads, self.hd, self.vocab, self.max_pos = heads, kv_heads, head_dim, vocab, max_pos
+        self.device = torch.device("cuda")
         g = torch.Generator(device="cuda").manual_seed(seed)
 
         def linear(n, k):  # held as MXFP4; this example multiplies with the values it stands for
@@ -68,34 +69,41 @@ def lookup_drafts(history, k):
 
 def serve(model, prompt, requests, n_tokens, draft, fmt="mxfp8", page=32, temperature=0.0, seed=0):
     """Continues `prompt` for every request (a list of its own first tokens).  Returns (tokens, target passes)."""
-    B, P = len(requests), len(prompt)
-    room = -(-(max(map(len, requests)) + n_tokens + draft + 2) // page)  # own pages per request
+    B, P, dev = len(requests), len(prompt), model.device
+    if not all(requests):
+        raise ValueError("every request needs a token of its own")
+    # A request may end with up to `draft` tokens more than it wanted, all but the last of them cached; while others go
+    # on, passes still write their 1 + draft rows after them.
+    most = max(map(len, requests)) + n_tokens + 2 * draft
+    if P + most > model.max_pos:
+        raise ValueError(f"{P + most} positions, and the model has {model.max_pos}")
+    room = -(-most // page)  # own pages per request
     shared = -(-P // page)
-    model.caches = [ops.MxKvCache.empty(shared + B * room, model.kv_heads, model.hd, page, fmt) for _ in model.layers]
-    prefix_pages = torch.arange(shared, dtype=torch.int32, device="cuda")
-    table = (shared + torch.arange(B * room, dtype=torch.int32, device="cuda")).view(B, room)
-    g = torch.Generator(device="cuda").manual_seed(seed)
+    model.caches = [ops.MxKvCache.empty(shared + B * room, model.kv_heads, model.hd, page, fmt, dev) for _ in model.layers]
+    prefix_pages = torch.arange(shared, dtype=torch.int32, device=dev)
+    table = (shared + torch.arange(B * room, dtype=torch.int32, device=dev)).view(B, room)
+    g = torch.Generator(device=dev).manual_seed(seed)
 
     # the prompt once, in passes of up to 64 tokens, as one sequence over the shared pages
     for at in range(0, P, 64):
-        part = torch.tensor([prompt[at:at + 64]], dtype=torch.int32, device="cuda")
+        part = torch.tensor([prompt[at:at + 64]], dtype=torch.int32, device=dev)
         t = part.shape[1]
-        pos = (at + torch.arange(t, device="cuda"))[None]
-        lens = torch.tensor([at + t], dtype=torch.int32, device="cuda")
+        pos = (at + torch.arange(t, device=dev))[None]
+        lens = torch.tensor([at + t], dtype=torch.int32, device=dev)
         model.forward(part, pos, pos.int(),
                       lambda i, q: ops.attn_paged_mx(model.caches[i], q, prefix_pages[None], lens))
 
     def step(new, own):
         """Runs new [B][t] after own[b] cached positions; returns the logits."""
         t = new.shape[1]
-        at = own[:, None] + torch.arange(t, device="cuda")
+        at = own[:, None] + torch.arange(t, device=dev)
         slots = (table.gather(1, (at // page).long()) * page + at % page).int()
         lens = (own + t).int()
         return model.forward(new, P + at, slots,
                              lambda i, q: ops.attn_shared_mx(model.caches[i], q, prefix_pages, P, table, lens))
 
     out = [list(r) for r in requests]
-    own = torch.zeros(B, dtype=torch.long, device="cuda")
+    own = torch.zeros(B, dtype=torch.long, device=dev)
     passes = 0
     while min(len(o) - len(r) for o, r in zip(out, requests)) < n_tokens:
         # tokens whose K/V are not cached yet, then the drafts; rows are padded to the longest
@@ -103,17 +111,17 @@ def serve(model, prompt, requests, n_tokens, draft, fmt="mxfp8", page=32, temper
         known = [o[d:] for o, d in zip(out, done)]
         drafts = [lookup_drafts(prompt + o, draft) if len(o) - len(r) < n_tokens else [] for o, r in zip(out, requests)]
         width = max(map(len, known)) + draft
-        rows = torch.tensor([(n + d + [0] * width)[:width] for n, d in zip(known, drafts)], dtype=torch.int32, device="cuda")
+        rows = torch.tensor([(n + d + [0] * width)[:width] for n, d in zip(known, drafts)], dtype=torch.int32, device=dev)
         logits = step(rows, own)
         passes += 1
-        first = torch.tensor([len(n) - 1 for n in known], device="cuda")
-        pick = logits.gather(1, (first[:, None] + torch.arange(draft + 1, device="cuda"))[..., None].expand(-1, -1, model.vocab))
+        first = torch.tensor([len(n) - 1 for n in known], device=dev)
+        pick = logits.gather(1, (first[:, None] + torch.arange(draft + 1, device=dev))[..., None].expand(-1, -1, model.vocab))
         accepted, tokens, _ = ops.verify_drafts(
-            pick, torch.tensor([(d + [0] * draft)[:draft] for d in drafts], dtype=torch.int32, device="cuda").view(B, draft),
-            torch.rand((B, draft), generator=g, device="cuda"),
-            torch.empty((B, model.vocab), device="cuda").exponential_(generator=g),
-            draft_lens=torch.tensor(list(map(len, drafts)), dtype=torch.int32, device="cuda"),
-            temperature=torch.full((B,), temperature, device="cuda"))
+            pick, torch.tensor([(d + [0] * draft)[:draft] for d in drafts], dtype=torch.int32, device=dev).view(B, draft),
+            torch.rand((B, draft), generator=g, device=dev),
+            torch.empty((B, model.vocab), device=dev).exponential_(generator=g),
+            draft_lens=torch.tensor(list(map(len, drafts)), dtype=torch.int32, device=dev),
+            temperature=torch.full((B,), temperature, device=dev))
         # the known tokens and the accepted drafts are cached now; rejected rows are overwritten later
         for b, (n, row) in enumerate(zip(accepted.tolist(), tokens.tolist())):
             if len(out[b]) - len(requests[b]) < n_tokens:
