@@ -237,10 +237,25 @@ def _f32(t: torch.Tensor, name: str):
     return _ptr(t)
 
 
-def _rows(t: torch.Tensor, n: int, name: str):
-    """Pointer and row stride of [rows][n] data whose leading dimension may be strided."""
-    if not t.is_cuda:
+def _together(first: torch.Tensor, *others):
+    """All tensors of a call (None: not given) lie on the current CUDA device."""
+    if not first.is_cuda:
         raise ValueError("fp4x operators take CUDA tensors (no CPU fallback)")
+    dev = first.get_device()
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in others:
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise ValueError(f"a tensor is on {t.device}, others of the call on cuda:{dev}")
+
+
+def _work(ws: torch.Tensor):
+    """Pointer and bytes of a workspace of any type."""
+    return _ptr(ws), ws.numel() * ws.element_size()
+
+
+def _rows(t: torch.Tensor, n: int):
+    """Pointer and row stride of [rows][n] data whose leading dimension may be strided."""
     return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else n)
 
 
@@ -253,6 +268,8 @@ class MxKvCache:
     """
 
     def __init__(self, k, k_scales, v, v_scales):
+        if k.dim() != 4 or k.shape[0] == 0:
+            raise ValueError("an MX cache is [n_pages][n_kv][page_size][row], with a page at least")
         n_pages, n_kv, page, row = k.shape
         head_dim = 32 * k_scales.shape[-1]
         if row not in (head_dim, head_dim // 2):
@@ -263,7 +280,7 @@ class MxKvCache:
         for t in (k, k_scales, v, v_scales):
             if t.dtype != torch.uint8 or not t.is_cuda or t.device != k.device:
                 raise ValueError("an MX cache is uint8 CUDA tensors of one device")
-            if n_pages and not t[0].is_contiguous():
+            if not t[0].is_contiguous():
                 raise ValueError("every page must be contiguous")
         if n_pages > 1 and (k.stride(0) != v.stride(0) or k_scales.stride(0) != v_scales.stride(0)):
             raise ValueError("K and V must have the same page stride")
@@ -288,6 +305,9 @@ class MxKvCache:
 
 def kv_append_mx(cache: MxKvCache, slots, k, v):
     """Quantise rows k, v [n][n_kv][head_dim] (f32 or bf16, rows may be strided) into the cache's slots [n] int32."""
+    _together(cache.k, slots, k, v)
+    if slots.dim() != 1:
+        raise ValueError("slots must be [n]")
     n = slots.shape[0]
     shape = (n, cache.n_kv, cache.head_dim)
     if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
@@ -297,12 +317,15 @@ def kv_append_mx(cache: MxKvCache, slots, k, v):
         if t.stride(2) != 1 or (t.stride(1) != hd and cache.n_kv > 1):
             raise ValueError("k and v rows must be contiguous")
     row = cache.n_kv * hd
-    (kp, ks), (vp, vs) = _rows(k, row, "k"), _rows(v, row, "v")
+    (kp, ks), (vp, vs) = _rows(k, row), _rows(v, row)
     check(lib().llama_kv_append_mx(_stream(), cache.ptr, n, _i32(slots, "slots"), _dtype(k), kp, ks, vp, vs))
 
 
 def kv_read_mx(cache: MxKvCache, slots, dtype=torch.bfloat16):
     """The cached rows in slots [n] int32 as K, V [n][n_kv][head_dim] of `dtype`; zeros for negative slots."""
+    _together(cache.k, slots)
+    if slots.dim() != 1:
+        raise ValueError("slots must be [n]")
     n = slots.shape[0]
     k, v = cache.k.new_empty((2, n, cache.n_kv, cache.head_dim), dtype=dtype).unbind(0)
     check(lib().llama_kv_read_mx(_stream(), cache.ptr, n, _i32(slots, "slots"), _dtype(k), k.data_ptr(), v.data_ptr()))
@@ -315,12 +338,11 @@ def attn_mx_workspace(cache: MxKvCache, batch, n_heads, q_len, prefix_len, max_l
     return cache.k.new_empty(max(nbytes, 16))
 
 
-def _attn_args(cache, q, page_table, lens, max_len):
+def _attn_args(cache, q, page_table, lens, max_len, *others):
+    _together(cache.k, q, page_table, lens, *others)
     if q.dim() != 4 or q.shape[3] != cache.head_dim:
         raise ValueError(f"q must be [batch][q_len][n_heads][{cache.head_dim}]")
     B, T, H, hd = q.shape
-    if not q.is_cuda:
-        raise ValueError("fp4x operators take CUDA tensors (no CPU fallback)")
     sb, st, sh, sd = q.stride()
     row = st if T > 1 else sb if B > 1 else H * hd
     if sd != 1 or (sh != hd and H > 1) or (B > 1 and sb != T * row):
@@ -335,25 +357,25 @@ def _attn_args(cache, q, page_table, lens, max_len):
 def attn_paged_mx(cache: MxKvCache, q, page_table, lens, max_len=None, workspace=None):
     """Attention of q [batch][q_len][n_heads][hd] over each sequence's own pages; lens [batch] int32 counts the cached
     positions with the q_len new ones as the last.  Returns a tensor shaped like q."""
-    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len)
+    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len, workspace)
     ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, 0, max_len)
     out = q.new_empty(q.shape)
     check(lib().llama_attn_paged_mx(_stream(), cache.ptr, B, H, T, _i32(page_table, "page_table"), page_table.shape[1],
                                     _i32(lens, "lens"), max_len, _dtype(q), q.data_ptr(), row, out.data_ptr(),
-                                    ws.data_ptr(), ws.numel()))
+                                    *_work(ws)))
     return out
 
 
 def attn_shared_mx(cache: MxKvCache, q, prefix_pages, prefix_len, page_table, lens, max_len=None, workspace=None):
     """attn_paged_mx for sequences that continue one prefix of prefix_len positions behind prefix_pages int32."""
-    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len)
+    B, T, H, row, max_len = _attn_args(cache, q, page_table, lens, max_len, prefix_pages, workspace)
     if prefix_pages.numel() * cache.page_size < prefix_len:
         raise ValueError("prefix_pages hold fewer than prefix_len positions")
     ws = workspace if workspace is not None else attn_mx_workspace(cache, B, H, T, prefix_len, max_len)
     out = q.new_empty(q.shape)
     check(lib().llama_attn_shared_mx(_stream(), cache.ptr, B, H, T, _i32(prefix_pages, "prefix_pages"), prefix_len,
                                      _i32(page_table, "page_table"), page_table.shape[1], _i32(lens, "lens"), max_len,
-                                     _dtype(q), q.data_ptr(), row, out.data_ptr(), ws.data_ptr(), ws.numel()))
+                                     _dtype(q), q.data_ptr(), row, out.data_ptr(), *_work(ws)))
     return out
 
 
@@ -363,6 +385,7 @@ def verify_drafts(logits, drafts, uniforms, noise, draft_probs=None, draft_lens=
     uniforms [batch][k], noise [batch][vocab] exponential draws, draft_probs [batch][k][vocab] (None: certain drafts),
     draft_lens [batch] int32, temperature [batch].  Returns (accepted [batch] int32, tokens [batch][k+1] int32,
     logprobs [batch][k+1])."""
+    _together(logits, drafts, uniforms, noise, draft_probs, draft_lens, temperature, workspace)
     B, K1, V = logits.shape
     k = K1 - 1
     if drafts.shape != (B, k) or uniforms.shape != (B, k) or noise.shape != (B, V):
@@ -372,7 +395,7 @@ def verify_drafts(logits, drafts, uniforms, noise, draft_probs=None, draft_lens=
     if (draft_lens is not None and draft_lens.shape != (B,)) or (temperature is not None and temperature.shape != (B,)):
         raise ValueError("verify_drafts: draft_lens and temperature must be [batch]")
     stride = logits.stride(1) if K1 > 1 else logits.stride(0) if B > 1 else V
-    if not logits.is_cuda or logits.stride(2) != 1 or (B > 1 and logits.stride(0) != K1 * stride):
+    if logits.stride(2) != 1 or (B > 1 and logits.stride(0) != K1 * stride):
         raise ValueError("verify_drafts: logits must be CUDA rows, evenly spaced")
     accepted, tokens = drafts.new_empty(B), drafts.new_empty((B, K1))
     logprobs = uniforms.new_empty((B, K1))
@@ -383,5 +406,5 @@ def verify_drafts(logits, drafts, uniforms, noise, draft_probs=None, draft_lens=
         None if draft_probs is None else _f32(draft_probs, "draft_probs"), _i32(drafts, "drafts"),
         None if draft_lens is None else _i32(draft_lens, "draft_lens"), _f32(uniforms, "uniforms"),
         _f32(noise, "noise"), None if temperature is None else _f32(temperature, "temperature"), accepted.data_ptr(),
-        tokens.data_ptr(), logprobs.data_ptr(), workspace.data_ptr(), workspace.numel()))
+        tokens.data_ptr(), logprobs.data_ptr(), *_work(workspace)))
     return accepted, tokens, logprobs
