@@ -10,9 +10,14 @@ import torch
 from . import MxKv, check, lib
 
 
+# The current device, and its stream's handle without building a torch.cuda.Stream (3 us per call): by torch's own cheap
+# calls where it has them.
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream():
-    # the current stream of the current device, without building a torch.cuda.Stream (3 us per call)
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(_device())
 
 
 def _ptr(t: torch.Tensor):
@@ -225,33 +230,36 @@ def _dtype(t: torch.Tensor) -> int:
     return d
 
 
+def _flat(t: torch.Tensor):
+    if not t.is_contiguous():
+        raise ValueError("fp4x operators take contiguous tensors")
+    return t.data_ptr()
+
+
+# of tensors that _together has seen
 def _i32(t: torch.Tensor, name: str):
     if t.dtype != torch.int32:
         raise ValueError(f"{name} must be int32, not {t.dtype}")
-    return _ptr(t)
+    return _flat(t)
 
 
 def _f32(t: torch.Tensor, name: str):
     if t.dtype != torch.float32:
         raise ValueError(f"{name} must be float32, not {t.dtype}")
-    return _ptr(t)
+    return _flat(t)
 
 
-def _together(first: torch.Tensor, *others):
+def _together(*tensors):
     """All tensors of a call (None: not given) lie on the current CUDA device."""
-    if not first.is_cuda:
-        raise ValueError("fp4x operators take CUDA tensors (no CPU fallback)")
-    dev = first.get_device()
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            raise ValueError(f"a tensor is on {t.device}, others of the call on cuda:{dev}")
+    dev = _device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"fp4x operators take CUDA tensors of the current device (cuda:{dev}), not {t.device}")
 
 
 def _work(ws: torch.Tensor):
     """Pointer and bytes of a workspace of any type."""
-    return _ptr(ws), ws.numel() * ws.element_size()
+    return _flat(ws), ws.numel() * ws.element_size()
 
 
 def _rows(t: torch.Tensor, n: int):

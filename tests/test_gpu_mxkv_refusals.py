@@ -86,3 +86,13 @@ def test_caches_without_pages_are_refused():
         ops.MxKvCache.empty(0, 2, 64, 16, "mxfp8")
     with pytest.raises(ValueError):
         ops.MxKvCache(*[torch.zeros((4, 16, 64), dtype=torch.uint8, device="cuda")] * 4)
+
+
+def test_stream_of_a_call(monkeypatch):
+    """The handle that the wrappers pass is the current stream's, with torch's private call and without it."""
+    side = torch.cuda.Stream()
+    for raw in (ops._raw_stream, None):
+        monkeypatch.setattr(ops, "_raw_stream", raw)
+        assert ops._stream() == torch.cuda.current_stream().cuda_stream
+        with torch.cuda.stream(side):
+            assert ops._stream() == side.cuda_stream
