@@ -274,12 +274,13 @@ FP4X_API size_t llama_attn_mx_workspace_size(const fp4x_mxkv *cache, uint32_t ba
  * 16-byte aligned.  Sequence b holds lens[b] positions (device array; clamped to
  * 0..max_len), the q_len query tokens of this step included as the last ones: query
  * i attends to positions 0 .. lens[b] - q_len + i; what the others hold (NaN
- * included) has no influence on it.  A query that sees no position gives zeros.  page_table [batch] rows of table_stride page ids, at least
+ * included) has no influence on it.  A query that sees no position gives zeros.
+ * page_table [batch] rows of table_stride page ids, at least
  * ceil(max_len / page_size) each; ids outside the cache are not read: their
  * positions are masked and the device error word is set.  Softmax scale
  * 1/sqrt(head_dim), statistics and sums in f32; the probabilities enter the tensor
  * cores with 16 bits (bf16 q) or 24 bits (f32 q, which itself enters with 22).
- * n_heads a multiple of n_kv_heads. */
+ * n_heads a multiple of n_kv_heads; q_len 1..64; lengths below 2^31 - 256. */
 FP4X_API int llama_attn_paged_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
                                  uint32_t q_len, const int32_t *page_table, uint32_t table_stride,
                                  const int32_t *lens, uint32_t max_len, uint32_t dtype, const void *q,
@@ -287,7 +288,8 @@ FP4X_API int llama_attn_paged_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, u
 /* The same for a batch whose sequences continue one shared prefix: every query sees
  * the prefix_len positions behind prefix_pages (device array of
  * ceil(prefix_len / page_size) ids) first, then its sequence's own positions as
- * above.  The prefix is read and dequantised once for the rows of all sequences. */
+ * above.  The prefix is read and dequantised once for every 128 rows (sequences x q_len x
+ * n_heads / n_kv_heads) of a KV head. */
 FP4X_API int llama_attn_shared_mx(fp4x_stream_t stream, const fp4x_mxkv *cache, uint32_t batch, uint32_t n_heads,
                                   uint32_t q_len, const int32_t *prefix_pages, uint32_t prefix_len,
                                   const int32_t *page_table, uint32_t table_stride, const int32_t *lens,

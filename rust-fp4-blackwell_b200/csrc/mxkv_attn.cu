@@ -1600,8 +1600,10 @@ int launch_attn(const char *who, cudaStream_t st, const fp4x_mxkv *cache, uint32
     FP4X_REQUIRE(n_heads && n_heads % p.c.n_kv == 0, "%s: n_heads %u is no multiple of n_kv_heads %u", who, n_heads,
                  p.c.n_kv);
     FP4X_REQUIRE(q_len >= 1 && q_len <= 64, "%s: q_len %u is not in 1..64", who, q_len);
-    FP4X_REQUIRE(max_len < 0x7FFFFFFFu && prefix_len < 0x7FFFFFFFu && max_len + prefix_len < 0x7FFFFFFFu,
-                 "%s: lengths must stay below 2^31", who);
+    // the end of the tile in which a sequence ends is a 32-bit signed position too
+    constexpr uint32_t kMost = 0x7FFFFFFFu - 2 * kChunk;
+    FP4X_REQUIRE(max_len <= kMost && prefix_len <= kMost && max_len + prefix_len <= kMost,
+                 "%s: lengths must stay below 2^31 - 256", who);
     if (batch == 0) return FP4X_OK;
     const uint64_t rows = (uint64_t)batch * q_len * n_heads;
     FP4X_REQUIRE(rows <= 0x3FFFFFFFull, "%s: too many query rows", who);

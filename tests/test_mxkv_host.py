@@ -135,3 +135,11 @@ def test_reference_verify_keeps_the_target_distribution():
     # binomial deviation: five standard deviations
     assert np.all(np.abs(got - p) <= 5 * np.sqrt(p * (1 - p) / n))
     assert abs(acc.mean() - np.minimum(p, q).sum()) <= 5 * 0.5 / np.sqrt(n)
+
+
+@pytest.mark.parametrize("own,prefix", [(0x7FFFFF80, 0), (0x7FFFFF00, 0), (0x7FFFFFFE, 0), (0, 0x7FFFFF80), (0x3FFFFFFF, 0x3FFFFFFF)],
+                         ids=str)
+def test_lengths_whose_last_tile_passes_31_bits_are_refused(own, prefix):
+    """A tile of up to 128 positions that starts below such a length ends past 2^31."""
+    assert _attn(_cache(), max_len=own, stride=1 << 26, prefix=64 if prefix else None, prefix_len=prefix) == 1
+    assert b"2^31" in fp4x.lib().fp4x_last_error()
