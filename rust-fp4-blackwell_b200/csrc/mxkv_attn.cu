@@ -56,7 +56,6 @@ struct AttnParams {
 __device__ __forceinline__ bool beside(const AttnParams &p, bool prefix) { return !prefix && p.prefix.ctas; }
 __device__ __forceinline__ void begin_kernel(const AttnParams &p, bool prefix) {
     if (!beside(p, prefix)) pdl_wait();
-    pdl_launch_dependents();
 }
 __device__ __forceinline__ void end_kernel(const AttnParams &p, bool prefix) {
     if (beside(p, prefix)) pdl_wait();
@@ -602,6 +601,7 @@ template <uint32_t FMT, uint32_t HD, uint32_t NQ, typename T>
 __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>::MIN_CTAS)
     attn_mx_kernel(const __grid_constant__ AttnParams p, bool prefix) {
     begin_kernel(p, prefix);
+    pdl_launch_dependents();
     constexpr bool F32 = sizeof(T) == 4;
     using TT = Tile<FMT, HD, NQ, F32>;
     using R = Ring<FMT, HD>;
@@ -983,6 +983,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
+    pdl_launch_dependents();  // not before this CTA has its tensor memory: a dependent may be this kernel again
     const uint32_t tmem = tmem_base;
     Segments segments(job, p.c.n_kv, loc);
     Segment sg = {};
@@ -1003,8 +1004,8 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             const uint32_t stop = min(sg.c1 * kChunk, sg.len);
             float m = kNoMax, l = 0.0f;
             bool good = true;
-            uint32_t done = 0;  // tiles of the segment so far
-            for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile, ++done) {
+            uint32_t taken = 0;  // tiles of the segment so far
+            for (uint32_t pos = sg.c0 * kChunk; pos < stop; pos += TN, ++tile, ++taken) {
                 const uint32_t buf = tile & 1, ph = (tile >> 1) & 1, sb = tmem + lanes + buf * BG::S_COLS;
                 good = good && warp_wait(&sfull[buf], ph);
                 tc::fence_after_sync();
@@ -1040,10 +1041,10 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
                 }
                 mx = fmaxf(mx, other) * p.scale;
                 const bool grow = mx > m + kLag, any = __any_sync(~0u, grow);
-                const bool flush = done && done % BG::FLUSH == 0, summed = done > BG::FLUSH;
+                const bool flush = taken && taken % BG::FLUSH == 0, summed = taken > BG::FLUSH;
                 const float mn = grow ? mx : m, f = any ? ex2(m - mn) : 1.0f;
                 m = mn, l *= f;
-                if ((any && done) || flush) {  // O rescaled, or moved to the sum
+                if ((any && taken) || flush) {  // O rescaled, or moved to the sum
                     const uint32_t pt = tile - 1;
                     good = warp_wait(&pvdone[pt & 1], (pt >> 1) & 1);
                     tc::fence_after_sync();
@@ -1125,7 +1126,7 @@ __global__ void __launch_bounds__(Big<HD, sizeof(T) == 4>::THREADS, 1)
             for (uint32_t c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
                 uint32_t x[32];
                 tmem_ld32(tmem + lanes + BG::O_COL + c * 32, x);
-                if (done > BG::FLUSH) {
+                if (taken > BG::FLUSH) {
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
                         uint32_t z[16];
