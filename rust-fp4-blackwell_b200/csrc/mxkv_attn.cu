@@ -1507,11 +1507,18 @@ __global__ void __launch_bounds__(128) attn_mx_join_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------- host
-// Rows of a tile: 8 per mma column tile; up to 32 rows share one read of the codes in
-// attn_mx_kernel, 128 in attn_mx_tile_kernel.  Measured on 24 sequences of up to 6001
-// positions, 4 KV heads x 64, MXFP4, f32 queries: 32 rows 47 us there; 40 rows 79 us there
-// as two tiles, 62 us on the tile kernel.
-inline uint32_t tile_rows_of(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
+// Rows of a tile: 8 per mma column tile; up to 32 rows share one read of the codes in attn_mx_kernel, 128 in
+// attn_mx_tile_kernel.  Time on the GPU of calls with MXFP8 (MXFP4 within 6 % of it), 4 KV heads, 24 sequences of up
+// to 6001 positions (in brackets one of 32768):
+//   rows                    20 or 40 in attn_mx_kernel     in attn_mx_tile_kernel
+//   40 x 64, bf16 / f32     72 (37) / 90 (40) us           52 (29) / 70 (37) us
+//   40 x 128, bf16 / f32    108 (47) / 135 (59)            62 (35) / 93 (47)
+//   20 x 64, bf16 / f32     45 (33) / 53 (29)              48 (29) / 66 (37)
+//   20 x 128, bf16 / f32    64 (33) / 77 (41)              58 (33) / 88 (46)
+inline uint32_t tile_rows_of(uint64_t rows, uint32_t hd, bool f32) {
+    const uint32_t most = hd == 128 && !f32 ? 16 : 32;
+    return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= most ? 32 : 128;
+}
 
 struct Plan {
     uint32_t own_rows, prefix_rows;  // per tile
@@ -1521,14 +1528,14 @@ struct Plan {
 // CTAs of a job that run at once per SM.
 inline uint32_t ctas_per_sm(uint32_t hd, uint32_t tile_rows, bool f32) { return two_ctas(tile_rows / 8 * hd, f32) ? 2 : 1; }
 
-// The plan for bf16 queries needs at least the workspace of that for f32 (it has at least the CTAs).
+// The plan for bf16 queries needs at least the workspace of that for f32 (it has at least the CTAs, and their rows).
 Plan make_plan(uint32_t n_kv, uint32_t hd, uint32_t batch, uint32_t n_heads, uint32_t q_len, uint32_t prefix_len,
                uint32_t max_len, bool f32) {
     Plan pl = {};
     const uint64_t rows = (uint64_t)(n_heads / n_kv) * q_len, all = rows * batch;
     const uint32_t sms = (uint32_t)num_sms();
     auto job = [&](uint32_t seqs, uint32_t len, uint64_t r, uint32_t &tile_rows, uint32_t &ctas, uint64_t &slots) {
-        tile_rows = tile_rows_of(r);
+        tile_rows = tile_rows_of(r, hd, f32);
         const uint64_t chunks = ((uint64_t)len + kChunk - 1) / kChunk * seqs * n_kv * ((r + tile_rows - 1) / tile_rows);
         const uint64_t room = (uint64_t)sms * ctas_per_sm(hd, tile_rows, f32);
         ctas = (uint32_t)(chunks < room ? chunks : room);  // more would idle
@@ -1579,10 +1586,14 @@ int launch_all(const char *who, cudaStream_t st, const AttnParams &p, uint64_t r
     for (int prefix = 1; prefix >= 0 && rc == FP4X_OK; --prefix) {
         const Job &job = prefix ? p.prefix : p.own;
         if (!job.ctas) continue;
-        rc = job.tile_rows == 8    ? launch_stream<FMT, HD, 1, T>(who, st, p, prefix)
-             : job.tile_rows == 16 ? launch_stream<FMT, HD, 2, T>(who, st, p, prefix)
-             : job.tile_rows == 32 ? launch_stream<FMT, HD, 4, T>(who, st, p, prefix)
-                                   : launch_tile<FMT, HD, T>(who, st, p, prefix);
+        if (job.tile_rows == 8)
+            rc = launch_stream<FMT, HD, 1, T>(who, st, p, prefix);
+        else if (job.tile_rows == 16)
+            rc = launch_stream<FMT, HD, 2, T>(who, st, p, prefix);
+        else if (job.tile_rows == 128)
+            rc = launch_tile<FMT, HD, T>(who, st, p, prefix);
+        else if constexpr (HD == 64 || sizeof(T) == 4)
+            rc = launch_stream<FMT, HD, 4, T>(who, st, p, prefix);
     }
     if (rc != FP4X_OK) return rc;
     const cudaError_t e = launch_pdl(attn_mx_join_kernel<FMT, HD, T>, dim3((uint32_t)rows), dim3(128), 0, st, p);
