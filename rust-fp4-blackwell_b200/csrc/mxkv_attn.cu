@@ -832,8 +832,10 @@ struct Big {
     static constexpr uint32_t S_COLS = F32 ? 96 : 128, O_COL = 2 * S_COLS, SUM_COL = O_COL + HD, COLS = 512;
     // O is added to a sum of its own every FLUSH tiles, because the MMA's accumulator cuts off what it adds (see
     // Tile::SUMS).  f32: 24 additions a time, 4.3e-7 of sums of one sign (every 8 tiles: 5.0e-6; every tile: 4.0e-7
-    // for up to 3 % of the time).  bf16: 128, a few 1e-6 (never: 1.5 % faster on 32768 positions).
-    static constexpr uint32_t FLUSH = F32 ? 2 : 8;
+    // for up to 3 % of the time).  bf16, 96 x 4 rows on 32768 positions: 64 additions, 0.12 % of the results on the other
+    // side of a rounding edge than the 64-bit ones (plain f32 arithmetic: 0.15 %); every 8 tiles 0.14 % and 2 % less
+    // time, every 2 tiles 0.11 % and 5 % more, never 0.3 % and 3.5 % less.
+    static constexpr uint32_t FLUSH = F32 ? 2 : 4;
     // first column of term z of P for positions 16 ks .. 16 ks + 15 (8 columns), from the buffer's start
     static __device__ __forceinline__ uint32_t p_col(uint32_t z, uint32_t ks) {
         return F32 ? 32 * z + 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks & 1);
