@@ -97,8 +97,8 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, flo
 // 2t and 2t + 1, dimensions 8t..8t+7 of every 32-block, so it moves 16-byte pieces on
 // both sides and a block's maximum takes two shuffles.  Bound by HBM: 131072 rows of
 // 8 x 128 MXFP8 to bf16 take 124 us (0.98 of the measured rate), 16384 bf16 rows to MXFP4
-// 19.8 us (85 MB, 4.3 TB/s), f32 rows to MXFP8 30.7 us (5.5 TB/s).  For MXFP4 the ALU came
-// first: 33 us with shuffles that name four lanes instead of the whole warp, 26 us with the
+// 19.8 us (85 MB, 4.3 TB/s), f32 rows to MXFP8 30.7 us (5.5 TB/s).  For MXFP4 the ALU comes
+// first (65 % busy at 2.64 instructions a cycle and SM): 33 us with shuffles that name four lanes instead of the whole warp, 26 us with the
 // f32 tie rule (below) for bf16 rows too.
 template <uint32_t HD>
 struct RowId {

@@ -818,9 +818,9 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
 //               through shared memory), exp2, row sum; P as two bf16 terms (16 bits; f32
 //               queries: Q and P as three, 24 bits) back into tensor memory, from where
 //               it is the A operand.  O is rescaled only when a row's maximum grows by
-//               more than kLag powers of two.
+//               more than kLag powers of two, and moved to a sum every FLUSH tiles.
 // Bound by the instructions of the two: 96 x 4 rows x 8 heads on 32768 positions (MXFP8,
-// bf16) take 113 us, 4300 cycles a tile, 1536 of them MMAs.
+// bf16) take 118 us, 4500 cycles a tile, 1536 of them MMAs.
 template <uint32_t HD, bool F32>
 struct Big {
     static constexpr uint32_t TN = F32 ? 64 : 128, QT = F32 ? 3 : 1, PT = F32 ? 3 : 2;
