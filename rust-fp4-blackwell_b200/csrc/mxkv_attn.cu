@@ -300,6 +300,9 @@ struct Tile {
     // keep the second CTA (184 us; 204 with one) and the chain: 2 additions a tile, up to 1e-4 of a result over 131072
     // positions in one CTA, where bf16 has steps of 4e-3 to 8e-3 of it.
     static constexpr bool SUMS = !(MIN_CTAS == 2 && NQ * HD == 256);
+    // The loop over the tiles in blocks of PERIOD, or a test in every tile: 222 against 231 us at 8 rows (as above), 288
+    // against 302 at 32 rows x 64, but 451 against 422 at 32 rows x 128 (f32 queries, 64 of up to 8192).
+    static constexpr bool BLOCKS = SUMS && (NQ == 1 || NQ * HD == 256);
     static constexpr uint32_t PERIOD = 16, SUM_BYTES = (SUMS ? NQ : 1) * MERGE_BYTES;
     static constexpr uint32_t STAGES = MIN_CTAS == 1 && NQ * HD == 256 ? 4 : R::STAGE > 3000 ? 2 : R::STAGE > 2000 ? 3 : 4;
     static constexpr uint32_t SMEM = kWarps * STAGES * R::STAGE + Q_BYTES + SUM_BYTES;
@@ -714,8 +717,9 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
         uint32_t stage = 0;
         bool summed = false;
         for (uint32_t j = 0; j < n_tiles;) {
-            const uint32_t to = TT::SUMS ? min(n_tiles, j + TT::PERIOD) : n_tiles;
+            const uint32_t to = TT::BLOCKS ? min(n_tiles, j + TT::PERIOD) : n_tiles;
             for (; j < to; ++j) {
+                if (TT::SUMS && !TT::BLOCKS && j && j % TT::PERIOD == 0) tile.to_sum(smem_u32(qbuf), summed), summed = true;
                 const uint32_t first = ((c0 + j) * kWarps + warp) * 16;
                 cp_async_wait<TT::STAGES - 1>();
                 __syncwarp();  // every lane's copies of the tile have landed
@@ -728,7 +732,7 @@ __global__ void __launch_bounds__(kWarps * 32, Tile<FMT, HD, NQ, sizeof(T) == 4>
                 __syncwarp();  // every lane has read the stage
                 issue(j + TT::STAGES);
             }
-            if (TT::SUMS && j < n_tiles) tile.to_sum(smem_u32(qbuf), summed), summed = true;
+            if (TT::BLOCKS && j < n_tiles) tile.to_sum(smem_u32(qbuf), summed), summed = true;
         }
         if (summed) tile.from_sum(smem_u32(qbuf));
         more = open(slot_of);  // its first copies run under the joining of this one
